@@ -21,6 +21,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # TORCH_MLU_AMD_ATEN_LIB: another build of the same extension (an instrumented one); there is still no fallback
 ATEN_LIB_PATH = os.environ.get("TORCH_MLU_AMD_ATEN_LIB") or os.path.join(_HERE, "lib", "libfa_aten.so")
 KERNEL_LIB_PATH = os.path.join(_HERE, "lib", "libfa_fwd.so")
+KV_LIB_PATH = os.path.join(_HERE, "lib", "libfa_kv.so")
 
 _loaded = False
 
@@ -30,7 +31,7 @@ def load() -> None:
     global _loaded
     if _loaded:
         return
-    for p in (KERNEL_LIB_PATH, ATEN_LIB_PATH):
+    for p in (KERNEL_LIB_PATH, KV_LIB_PATH, ATEN_LIB_PATH):
         if not os.path.exists(p):
             raise ImportError(
                 f"{p} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
@@ -43,20 +44,30 @@ load()
 
 from . import backends, capi  # noqa: E402
 from .ops import (  # noqa: E402
+    PagedPlan,
     flash_attention_forward,
     launch_count,
     paged_attention,
+    paged_cache_write,
+    paged_plan,
+    rotary,
+    rotary_frequencies,
     scaled_dot_product_flash_attention,
     sdpa,
 )
 
 __all__ = [
+    "PagedPlan",
     "backends",
     "capi",
     "flash_attention_forward",
     "launch_count",
     "load",
     "paged_attention",
+    "paged_cache_write",
+    "paged_plan",
+    "rotary",
+    "rotary_frequencies",
     "scaled_dot_product_flash_attention",
     "sdpa",
 ]

@@ -26,6 +26,7 @@ HIP_FLAGS = [
 
 
 KERNEL_SOURCES = ("fa_fwd_kernels.hip", "fa_bwd_kernels.hip")
+KV_SOURCES = ("fa_kv_kernels.hip", "fa_kv_attn_kernels.hip", "fa_rope_kernels.hip")
 
 
 def _run(cmd, **kw):
@@ -107,10 +108,40 @@ def build_kernels(verbose: bool = False) -> str:
     return out
 
 
+def build_kv(verbose: bool = False) -> str:
+    """hipcc: the paged 8-bit cache's and the rotary kernels -> lib/libfa_kv.so (the C ABI of include/fa_kv.h and
+    include/fa_rope.h)."""
+    os.makedirs(LIBDIR, exist_ok=True)
+    out = os.path.join(LIBDIR, "libfa_kv.so")
+    tmp = out + ".tmp"
+    objs = [os.path.join(LIBDIR, os.path.splitext(f)[0] + ".o") for f in KV_SOURCES]
+    procs = [(src, subprocess.Popen([HIPCC, *HIP_FLAGS, "-c", f"-I{INCLUDE}", f"-I{CSRC}", os.path.join(CSRC, src), "-o", obj],
+                                    stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+             for src, obj in zip(KV_SOURCES, objs)]
+    log = ""
+    for src, pr in procs:
+        o, _ = pr.communicate()
+        o = "\n".join(l for l in o.splitlines() if "is not a recognized feature for this target" not in l)
+        if pr.returncode != 0:
+            raise RuntimeError("build step failed: hipcc -c " + src + "\n" + o)
+        log += o
+    vs = os.path.join(LIBDIR, "kv_exports.map")
+    with open(vs, "w") as f:
+        f.write("{ global: fa_kv_*; fa_rope_*; local: *; };\n")
+    log += _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", f"-Wl,--version-script={vs}", *objs, "-o", tmp])
+    os.replace(tmp, out)
+    for f in (vs, *objs):
+        os.remove(f)
+    if verbose and log.strip():
+        print(log)
+    return out
+
+
 def build_aten(verbose: bool = False, out: str = None, extra_flags=()) -> str:
-    """g++: csrc/fa_aten.cpp + csrc/fa_sdp_choice.cpp -> lib/libfa_aten.so (registers the forward and backward aten ops
-    and the SDPA backend selector; links libfa_fwd.so by $ORIGIN).  `out` / `extra_flags`: an instrumented build next
-    to the real one (the sanitizer test), which finds libfa_fwd.so through an rpath to lib/."""
+    """g++: csrc/fa_aten.cpp + csrc/fa_sdp_choice.cpp + csrc/fa_kv_aten.cpp -> lib/libfa_aten.so (registers the forward and
+    backward aten ops, the SDPA backend selector and the cache's operators; links libfa_fwd.so and libfa_kv.so by $ORIGIN).
+    `out` / `extra_flags`: an instrumented build next to the real one (the sanitizer test), which finds them through an
+    rpath to lib/."""
     import torch
     from torch.utils import cpp_extension as ce
 
@@ -123,8 +154,8 @@ def build_aten(verbose: bool = False, out: str = None, extra_flags=()) -> str:
     cmd = [
         "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unused-function",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-        *inc, os.path.join(CSRC, "fa_aten.cpp"), os.path.join(CSRC, "fa_sdp_choice.cpp"), "-o", tmp,
-        f"-L{LIBDIR}", "-lfa_fwd", f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
+        *inc, *(os.path.join(CSRC, f) for f in ("fa_aten.cpp", "fa_sdp_choice.cpp", "fa_kv_aten.cpp")), "-o", tmp,
+        f"-L{LIBDIR}", "-lfa_fwd", "-lfa_kv", f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{LIBDIR}", f"-Wl,-rpath,{tlib}", "-Wl,--no-as-needed", *extra_flags,
     ]
     log = _run(cmd)
@@ -136,6 +167,7 @@ def build_aten(verbose: bool = False, out: str = None, extra_flags=()) -> str:
 
 def build_all(verbose: bool = False) -> None:
     build_kernels(verbose)
+    build_kv(verbose)
     build_aten(verbose)
 
 

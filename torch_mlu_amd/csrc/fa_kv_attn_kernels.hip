@@ -1,0 +1,506 @@
+// Attention over a paged cache of 8-bit values with a scale for each (block of tokens, kv head): the kernels and the C ABI of
+// fa_kv_attn_* (include/fa_kv.h).
+//
+//   S = Q K^T,  score = scale ks S,  P = exp(score - m),  O = sum_j P_j vs_j V_j / sum_j P_j,  lse = m + ln sum_j P_j
+//
+// K and V enter the matrix cores as bf16 / fp16, which hold every stored value exactly, and the scales of a block are one number
+// for 32 keys: ks multiplies the scores' exp2 factor, vs the probabilities before they are rounded.
+#include <hip/hip_runtime.h>
+
+#include "fa_kv_device.h"
+#include "fa_kv_host.h"
+
+namespace {
+using namespace fa;
+
+struct AArgs {
+  const unsigned char* q;
+  const unsigned char* k;
+  const unsigned char* v;
+  const float* ks;
+  const float* vs;
+  unsigned char* out;
+  float* lse;
+  const int32_t* table;
+  const int32_t* used;
+  const int32_t* cu_q;
+  int64_t q_sb, q_ss, q_sh;  // bytes
+  int64_t k_sp, k_ss, k_sh;
+  int64_t v_sp, v_ss, v_sh;
+  int64_t ks_sp, ks_sb, ks_sh;  // elements
+  int64_t vs_sp, vs_sb, vs_sh;
+  int64_t o_sb, o_ss, o_sh;        // bytes
+  int64_t lse_sb, lse_sh, lse_ss;  // elements
+  int64_t bt_stride;
+  int32_t batch, heads_q, heads_k, group;
+  int32_t seqlen_q, total_q, head_dim;
+  int32_t num_pages, table_pages, page_size;
+  int32_t page_blocks;      // 32-row blocks of a page
+  uint64_t scale_inv;       // ceil(2^32 / n) for scale blocks of n 32-row blocks: (block in the page * scale_inv) >> 32 is its scale
+  int32_t is_causal, neg_scale, n_splits, row_blocks;
+  float scale_log2;
+  float* ws_o;   // [batch * heads_q * seqlen_q * n_splits][head_dim]
+  float* ws_ml;  // [...][2]: maximum (log2 domain), sum
+};
+
+// Probabilities (at most 1) times this go into the second product: fp16 has 2^-14 as its smallest normal value, and a block
+// whose scale is far below the largest, or a key whose probability is, should not fall below it.
+template <typename T>
+constexpr float kLift = 1.0f;
+template <>
+constexpr float kLift<_Float16> = 32768.0f;
+
+// A wavefront streams 32-key blocks straight into registers, in the layouts that v_mfma_f32_16x16x32 wants:
+//   S^T (keys x rows) = K Q^T: lane (L, G) = (lane & 15, lane >> 4) holds key L's bytes 64 c + 16 G ... + 15, which are the
+//     contraction's elements of two steps; Q is laid out to match, as the order of a contraction is free.
+//   O^T (d x rows) = V^T P^T: lane (L, G) holds bytes VB L ... VB L + VB - 1 of the 8 keys 4 G + j and 16 + 4 G + j, j < 4,
+//     which are the keys of its own scores, so P needs no exchange; byte i of a lane goes to the product that makes rows
+//     d = VB L + i, and two keys' bytes are put side by side before they are converted.
+// So K and V pass through no LDS, every byte is read once in whole cache lines, and the four wavefronts of a workgroup, which
+// take turns in the key blocks, meet only at the end.
+template <typename T, int F, int DP, int CT>
+__global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP <= 128 ? 2 : 1)) fa_kv_attn_kernel(const AArgs a) {
+  constexpr int NW = 4;
+  constexpr int KC = DP / 64;  // 16-byte pieces of a key a lane holds
+  constexpr int KS = DP / 32;  // steps of the contraction over head_dim
+  constexpr int VB = DP / 16;  // bytes of a key of V a lane holds = 16-row blocks of O^T
+  constexpr int VW = VB / 4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int L = lane & 15, G = lane >> 4;
+
+  // workgroups that share K and V (the row blocks of one sequence, head and slice) are neighbours on one XCD: consecutive
+  // workgroups go round the 8 XCDs
+  const unsigned per = gridDim.x >> 3, w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  const unsigned unit = w / (unsigned)a.row_blocks;
+  const int rb = a.row_blocks - 1 - (int)(w - unit * a.row_blocks);
+  const unsigned bhk = unit / (unsigned)a.n_splits;
+  const int split = (int)(unit - bhk * a.n_splits);
+  const int b = (int)(bhk / (unsigned)a.heads_k), hk = (int)(bhk - (unsigned)b * a.heads_k);
+  if (b >= a.batch) return;  // the grid is rounded up to a multiple of 8
+
+  const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
+  const int R = rows.count * a.group, r0 = rb * 16 * CT;
+  if (r0 >= R) return;
+  const int Lk = min(max(a.used[b], 0), a.table_pages * a.page_size);
+  const int first_q = r0 / a.group, last_q = (min(r0 + 16 * CT, R) - 1) / a.group;
+  // row i of the sequence sees keys up to shift + i
+  const int shift = a.is_causal ? Lk - rows.aligned : 0x3fffffff;
+  const int mask_from = min(Lk, shift + first_q + 1);  // first key that some row does not see
+  const int keys = min(Lk, max(shift + last_q + 1, 0));
+
+  const int nblk = (keys + 31) >> 5;
+  const int per_split = (nblk + a.n_splits - 1) / a.n_splits;
+  const int blk_begin = split * per_split, blk_end = min(nblk, blk_begin + per_split);
+  const int blk0 = blk_begin + wave;
+  const int n_my = max(0, (blk_end - blk0 + NW - 1) / NW);
+
+  int lim[CT];  // the last key that this lane's row sees
+  s16x8 qf[CT][KS];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int r = r0 + 16 * ct + L;
+    const int qr = min(r, R - 1) / a.group, g = min(r, R - 1) - qr * a.group;
+    lim[ct] = min(Lk - 1, shift + qr);
+    const unsigned char* qp = a.q + (a.cu_q ? 0 : (int64_t)b * a.q_sb) + (int64_t)(rows.first + qr) * a.q_ss + (int64_t)(hk * a.group + g) * a.q_sh;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 64 * (s >> 1) + 16 * G + 8 * (s & 1);
+      u32x4 x = {0, 0, 0, 0};
+      if (r < R && d < a.head_dim) x = *(const u32x4*)(qp + d * 2);
+      if (a.neg_scale) x ^= 0x80008000u;
+      qf[ct][s] = __builtin_bit_cast(s16x8, x);
+    }
+  }
+
+  f32x4 o[VB][CT];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = -INFINITY;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VB; ++i) o[i][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // O is held in units of `ref`, the largest V scale so far, so that P vs / ref stays in fp16's range whatever the scales are
+  float ref = 1.17549435e-38f;
+
+  if (n_my > 0) {
+    ConstI32Ptr tbl = (ConstI32Ptr)(uintptr_t)(a.table + (int64_t)b * a.bt_stride);
+    const unsigned char* kh = a.k + (int64_t)hk * a.k_sh;
+    const unsigned char* vh = a.v + (int64_t)hk * a.v_sh;
+    ConstF32Ptr ksp = (ConstF32Ptr)(uintptr_t)(a.ks + (int64_t)hk * a.ks_sh);
+    ConstF32Ptr vsp = (ConstF32Ptr)(uintptr_t)(a.vs + (int64_t)hk * a.vs_sh);
+    const unsigned kss = (unsigned)a.k_ss, vss = (unsigned)a.v_ss;
+    int kd[KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) kd[c] = 64 * c + 16 * G < a.head_dim ? 64 * c + 16 * G : 0;
+    const int vd = VB * L < a.head_dim ? VB * L : 0;
+    const unsigned voff = 4 * G * vss + vd;
+    unsigned koff[KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) koff[c] = L * kss + kd[c];
+
+    int pg_idx = blk0 / a.page_blocks, pg_in = blk0 - pg_idx * a.page_blocks;
+    int page = tbl[pg_idx];
+
+    struct Block {
+      const unsigned char* k;
+      const unsigned char* v;
+      int left;      // last row that exists
+      bool hidden;   // its table entry names no page
+      float ks, vs;
+    };
+    // this wavefront's next block; the table entry of the one after it is requested
+    auto next_block = [&](int blk, bool more) -> Block {
+      Block x;
+      x.hidden = (unsigned)page >= (unsigned)a.num_pages;
+      const int64_t p = x.hidden ? 0 : page;
+      const unsigned row = (unsigned)pg_in * 32u;
+      const int64_t sb = (int64_t)(((uint64_t)(unsigned)pg_in * a.scale_inv) >> 32);
+      x.k = kh + p * a.k_sp + (uint64_t)row * kss;
+      x.v = vh + p * a.v_sp + (uint64_t)row * vss;
+      x.ks = ksp[p * a.ks_sp + sb * a.ks_sb];
+      x.vs = x.hidden ? 0.f : vsp[p * a.vs_sp + sb * a.vs_sb];
+      x.left = Lk - 1 - blk * 32;
+      pg_in += NW;
+      while (pg_in >= a.page_blocks) {
+        pg_in -= a.page_blocks;
+        ++pg_idx;
+      }
+      if (more) page = tbl[pg_idx];
+      return x;
+    };
+
+    u32x4 kr[2][KC];
+    unsigned vr[8][VW];
+    auto load_k = [&](const Block& x) {
+      if (x.left >= 31) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < KC; ++c) kr[t][c] = *(const u32x4*)(x.k + (uint64_t)(16u * t) * kss + koff[c]);
+      } else {  // the sequence's last block: rows clamped to its last one
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < KC; ++c) kr[t][c] = *(const u32x4*)(x.k + (unsigned)min(16 * t + L, x.left) * kss + kd[c]);
+      }
+    };
+    auto load_v = [&](const Block& x) {
+      auto get = [&](int j, const unsigned char* p) {
+        if constexpr (VW == 1) {
+          vr[j][0] = *(const unsigned*)p;
+        } else if constexpr (VW == 2) {
+          const u32x2 y = *(const u32x2*)p;
+          vr[j][0] = y[0];
+          vr[j][1] = y[1];
+        } else {
+          const u32x4 y = *(const u32x4*)p;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vr[j][i] = y[i];
+        }
+      };
+      if (x.left >= 31) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) get(j, x.v + (uint64_t)(unsigned)(j < 4 ? j : 12 + j) * vss + voff);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) get(j, x.v + (unsigned)min(4 * G + (j < 4 ? j : 12 + j), x.left) * vss + vd);
+      }
+    };
+
+    auto step = [&](const Block& x, int blk, auto&& after_k, auto&& after_v) {
+      f32x4 s[2][CT];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const unsigned w0 = kr[t][ks >> 1][2 * (ks & 1)], w1 = kr[t][ks >> 1][2 * (ks & 1) + 1];
+          const u32x4 f = {Stored<T, F>::template pair<0>(w0), Stored<T, F>::template pair<1>(w0),
+                           Stored<T, F>::template pair<0>(w1), Stored<T, F>::template pair<1>(w1)};
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) s[t][ct] = Mma<T>::m16(__builtin_bit_cast(s16x8, f), qf[ct][ks], s[t][ct]);
+        }
+      after_k();
+
+      // scale 0 (and a K scale of 0) must not meet the -inf of a masked score
+      const float c = fmaxf(a.scale_log2 * x.ks, 1e-30f);
+      if (blk * 32 + 32 > mask_from || x.hidden) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const int lm = x.hidden ? -1 : lim[ct] - blk * 32 - 4 * G;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (e > lm) s[0][ct][e] = -INFINITY;
+            if (16 + e > lm) s[1][ct][e] = -INFINITY;
+          }
+        }
+      }
+      if (x.vs > ref) {  // wavefront-uniform and rare
+        const float f = ref / x.vs;
+        ref = x.vs;
+#pragma unroll
+        for (int i = 0; i < VB; ++i)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) o[i][ct] *= f;
+      }
+      const float vf = x.vs / ref * kLift<T>;
+      if (x.hidden) {  // what was loaded in its place must not meet a probability of 0: it may be NaN
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 0; i < VW; ++i) vr[j][i] = 0;
+      }
+      s16x8 pb[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float mx = max3(s[0][ct][0], s[0][ct][1], s[0][ct][2]);
+        mx = max3(mx, s[0][ct][3], s[1][ct][0]);
+        mx = max3(mx, s[1][ct][1], s[1][ct][2]);
+        mx = max2(mx, s[1][ct][3]) * c;
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = pair_max32(mx);
+        if (__any(mx > m[ct])) {
+          const float mn = fmaxf(m[ct], mx);
+          const float f = mn == -INFINITY ? 1.f : fast_exp2(m[ct] - mn);
+          m[ct] = mn;
+          l[ct] *= f;
+#pragma unroll
+          for (int i = 0; i < VB; ++i) o[i][ct] *= f;
+        }
+        const float base = m[ct] == -INFINITY ? 0.f : m[ct];
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = fast_exp2(s[0][ct][e] * c - base);
+          p[4 + e] = fast_exp2(s[1][ct][e] * c - base);
+          l[ct] += p[e] + p[4 + e];
+        }
+        u32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = Mma<T>::pack2(p[2 * e] * vf, p[2 * e + 1] * vf);
+        pb[ct] = __builtin_bit_cast(s16x8, y);
+      }
+
+#pragma unroll
+      for (int wd = 0; wd < VW; ++wd)
+        static_for<0, 2>([&](auto H) {
+          constexpr int h = decltype(H)::value;
+          u32x4 fa, fb;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            // (key 2t, key 2t + 1) of byte 2h, then of byte 2h + 1
+            const unsigned z = __builtin_amdgcn_perm(vr[2 * t + 1][wd], vr[2 * t][wd], h ? 0x07030602u : 0x05010400u);
+            fa[t] = Stored<T, F>::template pair<0>(z);
+            fb[t] = Stored<T, F>::template pair<1>(z);
+          }
+          constexpr int i0 = 2 * h;
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            o[4 * wd + i0][ct] = Mma<T>::m16(__builtin_bit_cast(s16x8, fa), pb[ct], o[4 * wd + i0][ct]);
+            o[4 * wd + i0 + 1][ct] = Mma<T>::m16(__builtin_bit_cast(s16x8, fb), pb[ct], o[4 * wd + i0 + 1][ct]);
+          }
+        });
+      after_v();
+    };
+
+    Block x = next_block(blk0, n_my > 1);
+    load_k(x);
+    load_v(x);
+    int blk = blk0;
+    for (int it = 0; it + 1 < n_my; ++it, blk += NW) {
+      const Block y = next_block(blk + NW, it + 2 < n_my);
+      step(x, blk, [&] { load_k(y); }, [&] { load_v(y); });
+      x = y;
+    }
+    step(x, blk, [] {}, [] {});
+  }
+
+  // ---- the four wavefronts' partials, 16 rows at a time ----
+  constexpr int OS = DP + 4;
+  float* so = (float*)smem;                        // [NW][16][OS]
+  float* sml = (float*)(smem + NW * 16 * OS * 4);  // [NW][16][2]
+  const float o_unit = ref / kLift<T>;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (r0 + 16 * ct >= R) break;
+    float ls = l[ct];
+    ls += __shfl_xor(ls, 16);
+    ls = pair_sum32(ls);
+    if (ct) __syncthreads();
+    float* row = so + (wave * 16 + L) * OS;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < VB; i += 4) {
+        f32x4 y;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) y[z] = o[i + z][ct][e] * o_unit;
+        *(f32x4*)(row + VB * (4 * G + e) + i) = y;
+      }
+    if (G == 0) {
+      sml[(wave * 16 + L) * 2] = m[ct];
+      sml[(wave * 16 + L) * 2 + 1] = ls;
+    }
+    __syncthreads();
+    const int nrows = min(16, R - r0 - 16 * ct);
+    constexpr int TPR = DP / 4;
+    for (int item = tid; item < nrows * TPR; item += NW * 64) {
+      const int i = item / TPR, d = (item % TPR) * 4;
+      float mw[NW], M = -INFINITY;
+#pragma unroll
+      for (int y = 0; y < NW; ++y) {
+        mw[y] = sml[(y * 16 + i) * 2];
+        M = fmaxf(M, mw[y]);
+      }
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.f;
+#pragma unroll
+      for (int y = 0; y < NW; ++y) {
+        const float ly = sml[(y * 16 + i) * 2 + 1];
+        if (ly == 0.f) continue;  // a wavefront that saw no key of this row (a NaN goes on to the result)
+        const float f = fast_exp2(mw[y] - M);
+        sum += ly * f;
+        acc += *(const f32x4*)(so + (y * 16 + i) * OS + d) * f;
+      }
+      const int r = r0 + 16 * ct + i, qr = r / a.group, h = hk * a.group + r - qr * a.group;
+      if (a.n_splits == 1) {
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        if (d < a.head_dim) {
+          unsigned char* p = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(rows.first + qr) * a.o_ss + (int64_t)h * a.o_sh + d * 2;
+          *(u32x2*)p = u32x2{Mma<T>::pack2(acc[0] * inv, acc[1] * inv), Mma<T>::pack2(acc[2] * inv, acc[3] * inv)};
+        }
+        if (d == 0)
+          a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(rows.first + qr) * a.lse_ss] =
+              sum != 0.f ? (M + __builtin_log2f(sum)) * kLn2 : INFINITY;
+      } else {
+        const int64_t slot = (((int64_t)b * a.heads_q + h) * a.seqlen_q + qr) * a.n_splits + split;
+        if (d < a.head_dim) *(f32x4*)(a.ws_o + slot * a.head_dim + d) = acc;
+        if (d == 0) *(f32x2*)(a.ws_ml + slot * 2) = f32x2{M, sum};
+      }
+    }
+  }
+}
+
+// Joins the slices of a row: one wavefront a row, 4 elements of head_dim a lane, so that DP = 128 takes two slices at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= (int64_t)a.batch * a.heads_q * a.seqlen_q) return;
+  const int qr = (int)(r % a.seqlen_q), bh = (int)(r / a.seqlen_q);
+  const int h = bh % a.heads_q, b = bh / a.heads_q;
+  const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
+  if (qr >= rows.count) return;
+  const int D = a.head_dim, ns = a.n_splits;
+  const float* po = a.ws_o + r * ns * D;
+  f32x2 v = {-INFINITY, 0.f};
+  if (lane < ns) v = *(const f32x2*)(a.ws_ml + r * ns * 2 + 2 * lane);
+  float M = v[0];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+  const float f = v[1] == 0.f ? 0.f : fast_exp2(v[0] - M);
+  float sum = v[1] * f;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+  const int lps = D <= 64 ? 16 : (D <= 128 ? 32 : 64), spw = 64 / lps;
+  const int sub = lane / lps, d = (lane % lps) * 4;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < ns; s += spw) {
+    const int at = s + sub;
+    const float fs = __shfl(f, min(at, 63));
+    if (at < ns && d < D && fs > 0.f) acc += *(const f32x4*)(po + (int64_t)at * D + d) * fs;
+  }
+  for (int o = lps; o < 64; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o);
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  if (sub == 0 && d < D) {
+    unsigned char* p = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(rows.first + qr) * a.o_ss + (int64_t)h * a.o_sh + d * 2;
+    *(u32x2*)p = u32x2{Mma<T>::pack2(acc[0] * inv, acc[1] * inv), Mma<T>::pack2(acc[2] * inv, acc[3] * inv)};
+  }
+  if (lane == 0)
+    a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(rows.first + qr) * a.lse_ss] =
+        sum != 0.f ? (M + __builtin_log2f(sum)) * kLn2 : INFINITY;
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+using namespace fa::kvhost;
+
+template <typename T, int F, int DP, int CT>
+int launch_attn(const AArgs& a, hipStream_t st) {
+  constexpr int lds = 4 * 16 * ((DP + 4) * 4 + 8);
+  constexpr auto kfn = fa_kv_attn_kernel<T, F, DP, CT>;
+  if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
+  const int64_t n = (int64_t)a.batch * a.heads_k * a.n_splits * a.row_blocks;
+  if (n > 0x7ffffff0LL) return FA_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(kfn, dim3((unsigned)((n + 7) / 8 * 8)), dim3(256), lds, st, a);
+  if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
+  if (a.n_splits > 1) {
+    const int64_t rows = (int64_t)a.batch * a.heads_q * a.seqlen_q;
+    hipLaunchKernelGGL((fa_kv_merge_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
+  }
+  return FA_OK;
+}
+template <typename T, int F>
+int launch_attn(const AArgs& a, int tiles, hipStream_t st) {
+  if (a.head_dim <= 64) return tiles == 1 ? launch_attn<T, F, 64, 1>(a, st) : (tiles == 2 ? launch_attn<T, F, 64, 2>(a, st) : launch_attn<T, F, 64, 4>(a, st));
+  if (a.head_dim <= 128) return tiles == 1 ? launch_attn<T, F, 128, 1>(a, st) : (tiles == 2 ? launch_attn<T, F, 128, 2>(a, st) : launch_attn<T, F, 128, 4>(a, st));
+  return tiles == 1 ? launch_attn<T, F, 256, 1>(a, st) : launch_attn<T, F, 256, 2>(a, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_kv_attn_validate(const fa_kv_attn_params* p) { return attn_validate(p); }
+
+size_t fa_kv_attn_workspace_bytes(const fa_kv_attn_params* p) {
+  return attn_validate(p) == FA_OK ? attn_workspace_bytes(p, attn_plan(p)) : 0;
+}
+
+int fa_kv_attn_launch(const fa_kv_attn_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = attn_validate(p)) return rc;
+  const AttnPlan plan = attn_plan(p);
+  const size_t need = attn_workspace_bytes(p, plan);
+  if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return FA_ERR_BAD_ARG;
+  if (p->seqlen_q == 0 || (p->cu_seqlens_q && p->total_q == 0)) return FA_OK;
+  AArgs a;
+  a.q = (const unsigned char*)p->q; a.k = (const unsigned char*)p->key_pages; a.v = (const unsigned char*)p->value_pages;
+  a.ks = p->key_scales; a.vs = p->value_scales;
+  a.out = (unsigned char*)p->out; a.lse = p->lse;
+  a.table = p->block_table; a.used = p->seqused_k; a.cu_q = p->cu_seqlens_q;
+  a.q_sb = p->q_stride_b * 2; a.q_ss = p->q_stride_s * 2; a.q_sh = p->q_stride_h * 2;
+  a.k_sp = p->kp_stride_p; a.k_ss = p->kp_stride_s; a.k_sh = p->kp_stride_h;
+  a.v_sp = p->vp_stride_p; a.v_ss = p->vp_stride_s; a.v_sh = p->vp_stride_h;
+  a.ks_sp = p->ks_stride_p; a.ks_sb = p->ks_stride_b; a.ks_sh = p->ks_stride_h;
+  a.vs_sp = p->vs_stride_p; a.vs_sb = p->vs_stride_b; a.vs_sh = p->vs_stride_h;
+  a.o_sb = p->o_stride_b * 2; a.o_ss = p->o_stride_s * 2; a.o_sh = p->o_stride_h * 2;
+  a.lse_sb = p->lse_stride_b; a.lse_sh = p->lse_stride_h; a.lse_ss = p->lse_stride_s;
+  a.bt_stride = p->block_table_stride;
+  a.batch = p->batch; a.heads_q = p->heads_q; a.heads_k = p->heads_k; a.group = p->heads_q / p->heads_k;
+  a.seqlen_q = p->seqlen_q; a.total_q = p->total_q; a.head_dim = p->head_dim;
+  a.num_pages = p->num_pages; a.table_pages = p->table_pages; a.page_size = p->page_size;
+  a.page_blocks = p->page_size / 32;
+  const uint64_t sb = (uint64_t)p->scale_block / 32;  // exact: a page has at most 2^15 blocks
+  a.scale_inv = ((1ULL << 32) + sb - 1) / sb;
+  a.is_causal = p->is_causal; a.neg_scale = p->scale < 0.f ? 1 : 0;
+  a.n_splits = plan.splits; a.row_blocks = plan.row_blocks;
+  a.scale_log2 = fabsf(p->scale) * kLog2e;
+  a.ws_o = (float*)workspace;
+  a.ws_ml = a.ws_o + (need ? (size_t)p->batch * p->heads_q * p->seqlen_q * plan.splits * p->head_dim : 0);
+  hipStream_t st = (hipStream_t)stream;
+  if (p->dtype == FA_DTYPE_BF16)
+    return p->format == FA_KV_E4M3 ? launch_attn<__bf16, FA_KV_E4M3>(a, plan.tiles, st) : launch_attn<__bf16, FA_KV_INT8>(a, plan.tiles, st);
+  return p->format == FA_KV_E4M3 ? launch_attn<_Float16, FA_KV_E4M3>(a, plan.tiles, st) : launch_attn<_Float16, FA_KV_INT8>(a, plan.tiles, st);
+}
+
+}  // extern "C"
