@@ -7,6 +7,7 @@
 // for 32 keys: ks multiplies the scores' exp2 factor, vs the probabilities before they are rounded.
 #include <hip/hip_runtime.h>
 
+#include "fa_fwd_common.h"
 #include "fa_kv_device.h"
 #include "fa_kv_host.h"
 
@@ -49,6 +50,11 @@ template <typename T>
 constexpr float kLift = 1.0f;
 template <>
 constexpr float kLift<_Float16> = 32768.0f;
+// ... where a probability may be up to 2^kLazyLog2
+template <typename T>
+constexpr float kLazyLift = 1.0f;
+template <>
+constexpr float kLazyLift<_Float16> = 128.0f;
 
 // A wavefront streams 32-key blocks straight into registers, in the layouts that v_mfma_f32_16x16x32 wants:
 //   S^T (keys x rows) = K Q^T: lane (L, G) = (lane & 15, lane >> 4) holds key L's bytes 64 c + 16 G ... + 15, which are the
@@ -71,15 +77,15 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int L = lane & 15, G = lane >> 4;
 
-  // workgroups that share K and V (the row blocks of one sequence, head and slice) are neighbours on one XCD: consecutive
-  // workgroups go round the 8 XCDs
-  const unsigned per = gridDim.x >> 3, w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  const unsigned unit = w / (unsigned)a.row_blocks;
-  const int rb = a.row_blocks - 1 - (int)(w - unit * a.row_blocks);
+  // consecutive workgroups go round the 8 XCDs: those that share K and V (the row blocks of one sequence, head and slice) are
+  // neighbours on one, and a sequence's heads, whose lengths are the same, are spread over all
+  const unsigned turn = (blockIdx.x >> 3) / (unsigned)a.row_blocks;
+  const unsigned unit = turn * 8 + (blockIdx.x & 7);
+  const int rb = a.row_blocks - 1 - (int)((blockIdx.x >> 3) - turn * a.row_blocks);
   const unsigned bhk = unit / (unsigned)a.n_splits;
   const int split = (int)(unit - bhk * a.n_splits);
   const int b = (int)(bhk / (unsigned)a.heads_k), hk = (int)(bhk - (unsigned)b * a.heads_k);
-  if (b >= a.batch) return;  // the grid is rounded up to a multiple of 8
+  if (b >= a.batch) return;  // the grid has a multiple of 8 units
 
   const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
   const int R = rows.count * a.group, r0 = rb * 16 * CT;
@@ -389,6 +395,389 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
   }
 }
 
+// Many rows against the cache (chunks of prompts, packed batches): MFMA-bound.  One workgroup owns 128 (query row, head of the
+// group) pairs of one (sequence, kv head), 32 a wavefront, and goes through the keys in tiles of 64.  A tile is loaded into
+// registers while the one before it is computed, converted once for all four wavefronts and kept in LDS as bf16 / fp16, double
+// buffered; S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with one lane a row, as in the 16-bit tile kernel, whose LDS
+// layouts these are.  The heads of a group share the tile, so a conversion serves 4 x 32 rows instead of one wavefront's.
+template <typename T, int F, int DP>
+__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(const AArgs a) {
+  constexpr int ROWB = DP * 2;        // bytes of a row in LDS
+  constexpr int BM = 128, BN = 64;
+  constexpr int TILE = BN * ROWB;
+  constexpr int KS = DP / 16;         // steps of the contraction over head_dim
+  constexpr int MB = DP / 32;         // 32-row blocks of O^T
+  constexpr int PPR = DP / 16;        // 16-byte pieces of a stored row
+  constexpr int RPP = 256 / PPR;      // rows a pass of the workgroup loads
+  constexpr int NP = BN / RPP;        // passes a tile
+  constexpr int CPR = DP / 8;         // 16-byte chunks of a row in LDS
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // K0 K1 V0 V1
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, c32 = lane & 31;
+
+  const unsigned turn = (blockIdx.x >> 3) / (unsigned)a.row_blocks;  // as in fa_kv_attn_kernel
+  const unsigned unit = turn * 8 + (blockIdx.x & 7);
+  const int rb = a.row_blocks - 1 - (int)((blockIdx.x >> 3) - turn * a.row_blocks);
+  const unsigned bhk = unit / (unsigned)a.n_splits;
+  const int split = (int)(unit - bhk * a.n_splits);
+  const int b = (int)(bhk / (unsigned)a.heads_k), hk = (int)(bhk - (unsigned)b * a.heads_k);
+  if (b >= a.batch) return;
+
+  const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
+  const int R = rows.count * a.group, m0 = rb * BM;
+  if (m0 >= R) return;
+  const int Lk = min(max(a.used[b], 0), a.table_pages * a.page_size);
+  const int shift = a.is_causal ? Lk - rows.aligned : 0x3fffffff;
+  const int last_q = (min(m0 + BM, R) - 1) / a.group;
+  const int keys = min(Lk, max(shift + last_q + 1, 0));
+  const int all_tiles = (keys + BN - 1) / BN;
+  const int per_split = (all_tiles + a.n_splits - 1) / a.n_splits;
+  const int jt0 = split * per_split, ntiles = min(all_tiles, jt0 + per_split);
+
+  // this lane's row, and the span of its wavefront's
+  const int r = m0 + 32 * wave + c32;
+  const int qr = min(r, R - 1) / a.group, hg = min(r, R - 1) - qr * a.group;
+  const bool wave_live = m0 + 32 * wave < R;
+  const int lim_row = min(Lk - 1, shift + qr);
+  const int wave_lo = min(Lk - 1, shift + (m0 + 32 * wave) / a.group);                          // last key its first row sees
+  const int wave_hi = min(Lk - 1, shift + min(m0 + 32 * wave + 31, R - 1) / a.group);
+
+  // ---- the next tile: pages and scales of its two 32-key halves ----
+  ConstI32Ptr tbl = (ConstI32Ptr)(uintptr_t)(a.table + (int64_t)b * a.bt_stride);
+  const unsigned char* kh = a.k + (int64_t)hk * a.k_sh;
+  const unsigned char* vh = a.v + (int64_t)hk * a.v_sh;
+  ConstF32Ptr ksp = (ConstF32Ptr)(uintptr_t)(a.ks + (int64_t)hk * a.ks_sh);
+  ConstF32Ptr vsp = (ConstF32Ptr)(uintptr_t)(a.vs + (int64_t)hk * a.vs_sh);
+  const unsigned kss = (unsigned)a.k_ss, vss = (unsigned)a.v_ss;
+  struct Half32 {
+    const unsigned char* k;
+    const unsigned char* v;
+    int left;  // last row that exists
+    bool hidden;
+    float ks, vs;
+  };
+  int nb_idx = 0, nb_in = 0;  // the next 32-key block: entry of the table, block in its page
+  int page_a = 0, page_b = 0; // the entries of the next tile's halves
+  const int last_block = max(Lk - 1, 0) >> 5;
+  int nb = 0;                 // its number
+  auto seek = [&](int j) {
+    nb = 2 * j;
+    nb_idx = nb / a.page_blocks;
+    nb_in = nb - nb_idx * a.page_blocks;
+  };
+  auto request = [&]() {  // entries of the next tile (a half behind the last key has the other's)
+    page_a = tbl[min(nb, last_block) == nb ? nb_idx : 0];
+    const int next = nb_in + 1 >= a.page_blocks ? nb_idx + 1 : nb_idx;
+    page_b = nb + 1 <= last_block ? tbl[next] : page_a;
+  };
+  auto half = [&](int page, int in, int block) -> Half32 {
+    Half32 x;
+    x.hidden = (unsigned)page >= (unsigned)a.num_pages;
+    const int64_t p = x.hidden ? 0 : page;
+    const unsigned row = (unsigned)in * 32u;
+    const int64_t sb = (int64_t)(((uint64_t)(unsigned)in * a.scale_inv) >> 32);
+    x.k = kh + p * a.k_sp + (uint64_t)row * kss;
+    x.v = vh + p * a.v_sp + (uint64_t)row * vss;
+    x.ks = ksp[p * a.ks_sp + sb * a.ks_sb];
+    x.vs = x.hidden ? 0.f : vsp[p * a.vs_sp + sb * a.vs_sb];
+    x.left = Lk - 1 - block * 32;
+    return x;
+  };
+
+  const int pc = tid % PPR, prow = tid / PPR;
+  const int pd = pc * 16 < a.head_dim ? pc * 16 : 0;
+  u32x4 kraw[NP], vraw[NP];
+  Half32 h0, h1;
+  auto load_tile = [&]() {  // loads the next tile and moves on; nb is even
+    h0 = half(page_a, nb_in, nb);
+    int in1 = nb_in + 1, idx1 = nb_idx;
+    if (in1 >= a.page_blocks) {
+      in1 = 0;
+      ++idx1;
+    }
+    if (nb + 1 <= last_block) h1 = half(page_b, in1, nb + 1);
+    else h1 = h0;  // no key there: copies of rows that exist
+    nb += 2;
+    nb_idx = idx1;
+    nb_in = in1 + 1;
+    if (nb_in >= a.page_blocks) {
+      nb_in = 0;
+      ++nb_idx;
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const bool second = __builtin_amdgcn_readfirstlane(prow + RPP * i) >= 32;
+      const unsigned char* kb = second ? h1.k : h0.k;
+      const unsigned char* vb = second ? h1.v : h0.v;
+      const unsigned row = (unsigned)min((prow + RPP * i) & 31, second ? h1.left : h0.left);
+      kraw[i] = *(const u32x4*)(kb + row * kss + pd);
+      vraw[i] = *(const u32x4*)(vb + row * vss + pd);
+    }
+  };
+  int st_k[NP], st_v[NP];  // LDS offsets of this thread's pieces (the second chunk is at ^ 16)
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int row = prow + RPP * i;
+    st_k[i] = row * ROWB + ((2 * pc) ^ swzK<DP>(row)) * 16;
+    st_v[i] = 2 * TILE + row * ROWB + ((2 * pc) ^ swzV<DP>(row)) * 16;
+  }
+  auto convert = [](unsigned w0, unsigned w1) {
+    return u32x4{Stored<T, F>::template pair<0>(w0), Stored<T, F>::template pair<1>(w0), Stored<T, F>::template pair<0>(w1),
+                 Stored<T, F>::template pair<1>(w1)};
+  };
+  auto store_tile = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const bool second = __builtin_amdgcn_readfirstlane(prow + RPP * i) >= 32;
+      if (second ? h1.hidden : h0.hidden) vraw[i] = u32x4{0, 0, 0, 0};  // may be NaN, and must not meet a probability of 0
+      unsigned char* base = smem + buf * TILE;
+      *(u32x4*)(base + st_k[i]) = convert(kraw[i][0], kraw[i][1]);
+      *(u32x4*)(base + (st_k[i] ^ 16)) = convert(kraw[i][2], kraw[i][3]);
+      *(u32x4*)(base + st_v[i]) = convert(vraw[i][0], vraw[i][1]);
+      *(u32x4*)(base + (st_v[i] ^ 16)) = convert(vraw[i][2], vraw[i][3]);
+    }
+  };
+
+  if (ntiles > jt0) {
+    seek(jt0);
+    request();
+  }
+
+  // ---- Q through the K and V buffers: 64 rows in each pair of them, whole rows an instruction ----
+  int kaddr[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) kaddr[ks] = c32 * ROWB + (((2 * ks + g) ^ swzK<DP>(c32)) * 16);
+  s16x8 qf[KS];
+  {
+    const unsigned char* qb = a.q + (a.cu_q ? 0 : (int64_t)b * a.q_sb) + (int64_t)rows.first * a.q_ss + (int64_t)hk * a.group * a.q_sh;
+#pragma unroll
+    for (int i = 0; i < BM * CPR / 256; ++i) {
+      const int row = (i * 256 + tid) / CPR, ch = (i * 256 + tid) % CPR;
+      const int rr = min(m0 + row, R - 1), rq = rr / a.group, rh = rr - rq * a.group;
+      u32x4 x = {0, 0, 0, 0};
+      if (ch * 8 < a.head_dim) x = *(const u32x4*)(qb + (int64_t)rq * a.q_ss + (int64_t)rh * a.q_sh + ch * 16);
+      *(u32x4*)(smem + row * ROWB + ((ch ^ swzK<DP>(row)) * 16)) = x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      u32x4 x = *(const u32x4*)(smem + 32 * wave * ROWB + kaddr[ks]);
+      if (a.neg_scale) x ^= 0x80008000u;
+      qf[ks] = __builtin_bit_cast(s16x8, x);
+    }
+    __syncthreads();
+  }
+
+  const int L = lane & 15, G = lane >> 4;
+  const int v_row = 4 * g + (L >> 2);
+  int vaddr[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+    vaddr[mb] = v_row * ROWB + (L & 1) * 8 + (((4 * mb + 2 * (G & 1) + ((L & 3) >> 1)) ^ swzV<DP>(v_row)) * 16);
+  LDS_AS const unsigned char* kptr[KS];
+  LDS_AS const unsigned char* vptr[MB];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    kptr[ks] = (LDS_AS const unsigned char*)smem + kaddr[ks];
+    if constexpr (DP <= 128) asm volatile("" : "+v"(kptr[ks]));
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    vptr[mb] = (LDS_AS const unsigned char*)smem + 2 * TILE + vaddr[mb];
+    if constexpr (DP <= 128) asm volatile("" : "+v"(vptr[mb]));
+  }
+
+  f32x16 o[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
+  float m_run = -INFINITY, base_run = 0.f, l_run = 0.f;
+  float ref = 1.17549435e-38f;  // O is held in units of the largest V scale so far
+
+  auto tile = [&](int j, auto bufc) {
+    constexpr int BUF = decltype(bufc)::value;
+    __syncthreads();  // tile j is in LDS; everyone is done with the other buffer
+    const bool more = j + 1 < ntiles;
+    // scores are in units of c0 and c1 per 32 keys; scale 0 (and a K scale of 0) must not meet the -inf of a masked score
+    const float c0 = fmaxf(a.scale_log2 * h0.ks, 1e-30f), c1 = fmaxf(a.scale_log2 * h1.ks, 1e-30f);
+    const float vs0 = h0.vs, vs1 = h1.vs;
+    const bool hid0 = h0.hidden, hid1 = h1.hidden;
+    if (more) {
+      load_tile();
+      if (j + 2 < ntiles) request();
+    }
+    if (wave_live && j * BN <= wave_hi) {
+      f32x16 s0, s1;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) { s0[v] = 0.f; s1[v] = 0.f; }
+      {
+        s16x8 ka[2][2];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          ka[ks][0] = *(LDS_AS const s16x8*)(kptr[ks] + BUF * TILE);
+          ka[ks][1] = *(LDS_AS const s16x8*)(kptr[ks] + BUF * TILE + 32 * ROWB);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s0 = Mma<T>::m32(ka[ks & 1][0], qf[ks], s0);
+          s1 = Mma<T>::m32(ka[ks & 1][1], qf[ks], s1);
+          if (ks + 2 < KS) {
+            ka[ks & 1][0] = *(LDS_AS const s16x8*)(kptr[ks + 2] + BUF * TILE);
+            ka[ks & 1][1] = *(LDS_AS const s16x8*)(kptr[ks + 2] + BUF * TILE + 32 * ROWB);
+          }
+        }
+      }
+      if (j * BN + BN - 1 > wave_lo || hid0 || hid1) {
+        const int lim = lim_row - j * BN - 4 * g;
+        const int la = hid0 ? -1 : lim, lb = hid1 ? -1 : lim;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int e = 8 * (v >> 2) + (v & 3);
+          if (e > la) s0[v] = -INFINITY;
+          if (32 + e > lb) s1[v] = -INFINITY;
+        }
+      }
+      // the compiler waits for the matrix pipe only in front of instructions it knows: the first read of each product is a
+      // canonicalize, and the asm maxima depend on it
+      const float g0 = __builtin_canonicalizef(s0[15]);
+      float x0 = max3d(s0[0], s0[1], s0[2], g0), x1 = max3d(s0[8], s0[9], s0[10], g0);
+#pragma unroll
+      for (int v = 3; v < 7; v += 2) {
+        x0 = max3(x0, s0[v], s0[v + 1]);
+        x1 = max3(x1, s0[v + 8], s0[v + 9]);
+      }
+      x0 = max3(x0, s0[7], g0);
+      const float g1 = __builtin_canonicalizef(s1[15]);
+      float x2 = max3d(s1[0], s1[1], s1[2], g1), x3 = max3d(s1[8], s1[9], s1[10], g1);
+#pragma unroll
+      for (int v = 3; v < 7; v += 2) {
+        x2 = max3(x2, s1[v], s1[v + 1]);
+        x3 = max3(x3, s1[v + 8], s1[v + 9]);
+      }
+      x2 = max3(x2, s1[7], g1);
+      const float mx = pair_max32(fmaxf(max2(x0, x1) * c0, max2(x2, x3) * c1));
+      const bool grow = mx > m_run + kLazyLog2;
+      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+        const float f = grow ? fast_exp2(m_run - mx) : 1.0f;  // exp2(-inf) = 0 on the first tile
+        m_run = grow ? mx : m_run;
+        base_run = m_run == -INFINITY ? 0.f : m_run;
+        l_run *= f;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[i][v] *= f;
+      }
+      const float top = fmaxf(vs0, vs1);
+      if (top > ref) {  // workgroup-uniform and rare
+        const float f = ref / top;
+        ref = top;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[i][v] *= f;
+      }
+      // The V scale of 32 keys enters as an addend of their exponents, and is divided out of their sum again: two
+      // instructions instead of one for each probability.  A scale that is 0 or next to it becomes 2^-60 of the largest,
+      // where it cannot be seen.
+      const float vf0 = fmaxf(vs0 / ref, 8.67361738e-19f), vf1 = fmaxf(vs1 / ref, 8.67361738e-19f);
+      const float b0 = base_run - __builtin_amdgcn_logf(vf0 * kLazyLift<T>), b1 = base_run - __builtin_amdgcn_logf(vf1 * kLazyLift<T>);
+      const float u0 = 1.f / (vf0 * kLazyLift<T>), u1 = 1.f / (vf1 * kLazyLift<T>);
+
+      auto vfrag = [&](int mb, int t) {
+        const s16x4 lo = lds_read_tr_lds(vptr[mb] + BUF * TILE + (16 * t) * ROWB);
+        const s16x4 hi = lds_read_tr_lds(vptr[mb] + BUF * TILE + (16 * t + 8) * ROWB);
+        return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      };
+      s16x8 va[2][MB];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) va[0][mb] = vfrag(mb, 0);
+      float rs[2] = {0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (t + 1 < 4) {
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) va[(t + 1) & 1][mb] = vfrag(mb, t + 1);
+        }
+        u32x4 y;
+#pragma unroll
+        for (int e2 = 0; e2 < 4; ++e2) {
+          const int v = 8 * (t & 1) + 2 * e2;
+          const float p0 = t < 2 ? fast_exp2(s0[v] * c0 - b0) : fast_exp2(s1[v] * c1 - b1);
+          const float p1 = t < 2 ? fast_exp2(s0[v + 1] * c0 - b0) : fast_exp2(s1[v + 1] * c1 - b1);
+          rs[t >> 1] += p0 + p1;
+          y[e2] = Mma<T>::pack2(p0, p1);
+        }
+        const s16x8 pb = __builtin_bit_cast(s16x8, y);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) o[mb] = Mma<T>::m32(va[t & 1][mb], pb, o[mb]);
+      }
+      l_run += rs[0] * u0 + rs[1] * u1;
+    }
+    if (more) store_tile(BUF ^ 1);
+  };
+
+  if (ntiles > jt0) {
+    load_tile();
+    if (jt0 + 1 < ntiles) request();
+    store_tile(0);
+    int j = jt0;
+    for (; j + 1 < ntiles; j += 2) {
+      tile(j, IC<0>{});
+      tile(j + 1, IC<1>{});
+    }
+    if (j < ntiles) tile(j, IC<0>{});
+  }
+
+  // ---- epilogue ----
+  l_run = pair_sum32(l_run);
+  const float o_unit = ref / kLazyLift<T>;
+  if (a.n_splits > 1) {
+    if (r < R) {
+      const int64_t slot = (((int64_t)b * a.heads_q + hk * a.group + hg) * a.seqlen_q + qr) * a.n_splits + split;
+      float* dst = a.ws_o + slot * a.head_dim;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int v4 = 0; v4 < 4; ++v4) {
+          const int d = 32 * mb + 8 * v4 + 4 * g;
+          if (d < a.head_dim)
+            *(f32x4*)(dst + d) = f32x4{o[mb][4 * v4] * o_unit, o[mb][4 * v4 + 1] * o_unit, o[mb][4 * v4 + 2] * o_unit, o[mb][4 * v4 + 3] * o_unit};
+        }
+      if (g == 0) *(f32x2*)(a.ws_ml + slot * 2) = f32x2{m_run, l_run};
+    }
+    return;
+  }
+  const float inv = l_run != 0.f ? o_unit / l_run : 0.f;
+  __syncthreads();  // every wavefront is done with the tiles
+  // whole rows go out: staged through LDS, each wavefront its own 32 rows
+  constexpr int OSTR = ROWB + 16;
+  unsigned char* stage = smem + wave * (32 * OSTR);
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int v4 = 0; v4 < 4; ++v4)
+      *(u32x2*)(stage + c32 * OSTR + (32 * mb + 8 * v4 + 4 * g) * 2) =
+          u32x2{Mma<T>::pack2(o[mb][4 * v4] * inv, o[mb][4 * v4 + 1] * inv), Mma<T>::pack2(o[mb][4 * v4 + 2] * inv, o[mb][4 * v4 + 3] * inv)};
+  constexpr int RPS = 64 / CPR;
+  const int sr = lane / CPR, sch = lane % CPR;
+  unsigned char* ob = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)rows.first * a.o_ss + (int64_t)hk * a.group * a.o_sh;
+#pragma unroll
+  for (int i = 0; i < 32 / RPS; ++i) {
+    const int rl = i * RPS + sr, rr = m0 + 32 * wave + rl;
+    const u32x4 x = *(const u32x4*)(stage + rl * OSTR + sch * 16);
+    if (rr < R && sch * 8 < a.head_dim) {
+      const int rq = rr / a.group, rh = rr - rq * a.group;
+      *(u32x4*)(ob + (int64_t)rq * a.o_ss + (int64_t)rh * a.o_sh + sch * 16) = x;
+    }
+  }
+  if (r < R && g == 0)
+    a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)(hk * a.group + hg) * a.lse_sh + (int64_t)(rows.first + qr) * a.lse_ss] =
+        l_run != 0.f ? (m_run + __builtin_log2f(l_run)) * kLn2 : INFINITY;
+}
+
 // Joins the slices of a row: one wavefront a row, 4 elements of head_dim a lane, so that DP = 128 takes two slices at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
@@ -434,24 +823,39 @@ __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
 // ---- host ---------------------------------------------------------------------------------------------------------------
 using namespace fa::kvhost;
 
+int64_t grid_of(const AArgs& a) { return ((int64_t)a.batch * a.heads_k * a.n_splits + 7) / 8 * 8 * a.row_blocks; }
+
+template <typename T>
+int launch_merge(const AArgs& a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.batch * a.heads_q * a.seqlen_q;
+  hipLaunchKernelGGL((fa_kv_merge_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
 template <typename T, int F, int DP, int CT>
 int launch_attn(const AArgs& a, hipStream_t st) {
   constexpr int lds = 4 * 16 * ((DP + 4) * 4 + 8);
   constexpr auto kfn = fa_kv_attn_kernel<T, F, DP, CT>;
   if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
-  const int64_t n = (int64_t)a.batch * a.heads_k * a.n_splits * a.row_blocks;
-  if (n > 0x7ffffff0LL) return FA_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(kfn, dim3((unsigned)((n + 7) / 8 * 8)), dim3(256), lds, st, a);
+  const int64_t n = grid_of(a);
+  if (n > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(kfn, dim3((unsigned)n), dim3(256), lds, st, a);
   if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
-  if (a.n_splits > 1) {
-    const int64_t rows = (int64_t)a.batch * a.heads_q * a.seqlen_q;
-    hipLaunchKernelGGL((fa_kv_merge_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
-    if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
-  }
-  return FA_OK;
+  return a.n_splits > 1 ? launch_merge<T>(a, st) : FA_OK;
+}
+template <typename T, int F, int DP>
+int launch_tile(const AArgs& a, hipStream_t st) {
+  constexpr int lds = 4 * 64 * DP * 2;
+  constexpr auto kfn = fa_kv_tile_kernel<T, F, DP>;
+  if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
+  const int64_t n = grid_of(a);
+  if (n > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(kfn, dim3((unsigned)n), dim3(256), lds, st, a);
+  if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
+  return a.n_splits > 1 ? launch_merge<T>(a, st) : FA_OK;
 }
 template <typename T, int F>
 int launch_attn(const AArgs& a, int tiles, hipStream_t st) {
+  if (tiles == 8) return a.head_dim <= 64 ? launch_tile<T, F, 64>(a, st) : (a.head_dim <= 128 ? launch_tile<T, F, 128>(a, st) : launch_tile<T, F, 256>(a, st));
   if (a.head_dim <= 64) return tiles == 1 ? launch_attn<T, F, 64, 1>(a, st) : (tiles == 2 ? launch_attn<T, F, 64, 2>(a, st) : launch_attn<T, F, 64, 4>(a, st));
   if (a.head_dim <= 128) return tiles == 1 ? launch_attn<T, F, 128, 1>(a, st) : (tiles == 2 ? launch_attn<T, F, 128, 2>(a, st) : launch_attn<T, F, 128, 4>(a, st));
   return tiles == 1 ? launch_attn<T, F, 256, 1>(a, st) : launch_attn<T, F, 256, 2>(a, st);

@@ -96,22 +96,27 @@ inline int attn_validate(const fa_kv_attn_params* p) {
 
 // How the call is cut: 16 * tiles (query row, head of the group) pairs a workgroup, `splits` slices of the key range.
 struct AttnPlan {
-  int32_t tiles;      // 1, 2 or 4 tiles of 16 rows
+  int32_t tiles;      // 1, 2 or 4 tiles of 16 rows: the streaming kernel; 8: the tile kernel
   int32_t row_blocks; // workgroups that share a (sequence, kv head, slice)
   int32_t splits;
 };
 inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
   AttnPlan r;
   const int64_t rows = (int64_t)p->seqlen_q * (p->heads_q / p->heads_k);
-  r.tiles = rows <= 16 ? 1 : (rows <= 32 || p->head_dim > 128 ? 2 : 4);
+  r.tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 && p->head_dim <= 128 ? 4 : 8));
   r.row_blocks = (int32_t)((rows + 16 * r.tiles - 1) / (16 * r.tiles));
   if (r.row_blocks < 1) r.row_blocks = 1;
-  const int64_t keys = (int64_t)p->table_pages * p->page_size, blocks = (keys + 31) / 32;
+  const int64_t keys = (int64_t)p->table_pages * p->page_size;
+  const int64_t blocks = r.tiles == 8 ? (keys + 63) / 64 : (keys + 31) / 32;
   const int64_t units = (int64_t)p->batch * p->heads_k * r.row_blocks;
   int64_t n = p->num_splits;
   if (n == 0) {
     n = 1;
-    while (n * 2 <= FA_MAX_SPLITS && units * n * 2 <= 1024 && keys / (n * 2) >= 256) n *= 2;
+    if (r.tiles == 8) {
+      while (n * 2 <= FA_MAX_SPLITS && units * n * 2 <= 512 && blocks / (n * 2) >= 16) n *= 2;
+    } else {
+      while (n * 2 <= FA_MAX_SPLITS && units * n * 2 <= 1024 && keys / (n * 2) >= 256) n *= 2;
+    }
   }
   if (n > blocks) n = blocks > 0 ? blocks : 1;
   // partial sums within 1 GiB
