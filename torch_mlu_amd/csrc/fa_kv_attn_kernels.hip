@@ -37,7 +37,7 @@ struct AArgs {
   int32_t seqlen_q, total_q, head_dim;
   int32_t num_pages, table_pages, page_size;
   int32_t page_blocks;      // 32-row blocks of a page
-  uint64_t scale_inv;       // ceil(2^32 / n) for scale blocks of n 32-row blocks: (block in the page * scale_inv) >> 32 is its scale
+  uint32_t scale_inv;       // ceil(2^31 / n) for scale blocks of n 32-row blocks: (block in the page * scale_inv) >> 31 is its scale
   int32_t is_causal, neg_scale, n_splits, row_blocks;
   float scale_log2;
   float* ws_o;   // [batch * heads_q * seqlen_q * n_splits][head_dim]
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
       x.hidden = (unsigned)page >= (unsigned)a.num_pages;
       const int64_t p = x.hidden ? 0 : page;
       const unsigned row = (unsigned)pg_in * 32u;
-      const int64_t sb = (int64_t)(((uint64_t)(unsigned)pg_in * a.scale_inv) >> 32);
+      const int64_t sb = (int64_t)(((uint64_t)(unsigned)pg_in * a.scale_inv) >> 31);
       x.k = kh + p * a.k_sp + (uint64_t)row * kss;
       x.v = vh + p * a.v_sp + (uint64_t)row * vss;
       x.ks = ksp[p * a.ks_sp + sb * a.ks_sb];
@@ -400,6 +400,20 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
 // registers while the one before it is computed, converted once for all four wavefronts and kept in LDS as bf16 / fp16, double
 // buffered; S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with one lane a row, as in the 16-bit tile kernel, whose LDS
 // layouts these are.  The heads of a group share the tile, so a conversion serves 4 x 32 rows instead of one wavefront's.
+// A copy of a kernel argument that the compiler takes for a value of its own: loaded in groups of eight, arguments are also kept
+// (and spilled) in groups of eight.
+__device__ __forceinline__ unsigned own(unsigned x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+// The arguments once more, read where they are used: what the end needs is not kept through the loop.
+typedef const __attribute__((address_space(4))) AArgs* ArgsPtr;
+__device__ __forceinline__ ArgsPtr args_again() {
+  ArgsPtr p = (ArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 template <typename T, int F, int DP>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(const AArgs a) {
   constexpr int ROWB = DP * 2;        // bytes of a row in LDS
@@ -445,76 +459,103 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   const int wave_hi = min(Lk - 1, shift + min(m0 + 32 * wave + 31, R - 1) / a.group);
 
   // ---- the next tile: pages and scales of its two 32-key halves ----
-  ConstI32Ptr tbl = (ConstI32Ptr)(uintptr_t)(a.table + (int64_t)b * a.bt_stride);
+  // Table entries (of the tile after the next) and scales (of the next) come by vector loads together with K and V, and are
+  // moved to scalar registers when those have landed: as scalar loads they share a counter with LDS reads, and every tile
+  // began with waiting for them.
+  const int32_t* tbl = a.table + (int64_t)b * a.bt_stride;
   const unsigned char* kh = a.k + (int64_t)hk * a.k_sh;
   const unsigned char* vh = a.v + (int64_t)hk * a.v_sh;
-  ConstF32Ptr ksp = (ConstF32Ptr)(uintptr_t)(a.ks + (int64_t)hk * a.ks_sh);
-  ConstF32Ptr vsp = (ConstF32Ptr)(uintptr_t)(a.vs + (int64_t)hk * a.vs_sh);
-  const unsigned kss = (unsigned)a.k_ss, vss = (unsigned)a.v_ss;
-  struct Half32 {
-    const unsigned char* k;
-    const unsigned char* v;
-    int left;  // last row that exists
-    bool hidden;
-    float ks, vs;
-  };
-  int nb_idx = 0, nb_in = 0;  // the next 32-key block: entry of the table, block in its page
-  int page_a = 0, page_b = 0; // the entries of the next tile's halves
-  const int last_block = max(Lk - 1, 0) >> 5;
-  int nb = 0;                 // its number
-  auto seek = [&](int j) {
-    nb = 2 * j;
-    nb_idx = nb / a.page_blocks;
-    nb_in = nb - nb_idx * a.page_blocks;
-  };
-  auto request = [&]() {  // entries of the next tile (a half behind the last key has the other's)
-    page_a = tbl[min(nb, last_block) == nb ? nb_idx : 0];
-    const int next = nb_in + 1 >= a.page_blocks ? nb_idx + 1 : nb_idx;
-    page_b = nb + 1 <= last_block ? tbl[next] : page_a;
-  };
-  auto half = [&](int page, int in, int block) -> Half32 {
-    Half32 x;
-    x.hidden = (unsigned)page >= (unsigned)a.num_pages;
-    const int64_t p = x.hidden ? 0 : page;
-    const unsigned row = (unsigned)in * 32u;
-    const int64_t sb = (int64_t)(((uint64_t)(unsigned)in * a.scale_inv) >> 32);
-    x.k = kh + p * a.k_sp + (uint64_t)row * kss;
-    x.v = vh + p * a.v_sp + (uint64_t)row * vss;
-    x.ks = ksp[p * a.ks_sp + sb * a.ks_sb];
-    x.vs = x.hidden ? 0.f : vsp[p * a.vs_sp + sb * a.vs_sb];
-    x.left = Lk - 1 - block * 32;
-    return x;
-  };
-
+  const float* ksp = a.ks + (int64_t)hk * a.ks_sh;
+  const float* vsp = a.vs + (int64_t)hk * a.vs_sh;
+  const unsigned kss = own((unsigned)a.k_ss), vss = own((unsigned)a.v_ss);
+  const unsigned k_sp = own((unsigned)a.k_sp), v_sp = own((unsigned)a.v_sp), ks_sp = own((unsigned)a.ks_sp), vs_sp = own((unsigned)a.vs_sp);
+  const unsigned ks_sb = own((unsigned)a.ks_sb), vs_sb = own((unsigned)a.vs_sb), scale_inv = own(a.scale_inv);
+  const unsigned num_pages = own((unsigned)a.num_pages);
+  const int page_blocks = (int)own((unsigned)a.page_blocks);
+  int zero;  // keeps the loads at wavefront-uniform addresses vector loads
+  asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+  const int last_block = max(Lk - 1, 0) >> 5, last_entry = last_block / page_blocks;
+  int nb = 2 * jt0;                                    // the next tile's first 32-key block,
+  int nb_idx = nb / page_blocks, nb_in = nb - nb_idx * page_blocks;  // its entry of the table and place in the page
+  int page0 = 0, page1 = 0;                            // the next tile's entries
+  bool hid0 = false, hid1 = false;                     // the current tile's: the entry names no page
+  bool next_hid0 = false, next_hid1 = false;
+  float sk0 = 0.f, sk1 = 0.f, sv0 = 0.f, sv1 = 0.f;    // the current tile's scales
+  float nk0 = 0.f, nk1 = 0.f, nv0 = 0.f, nv1 = 0.f;    // the next tile's, in flight
+  int in_flight0 = 0, in_flight1 = 0;                  // entries of the tile after that, in flight
+  // loads nb's tile and the entries of the one after it
   const int pc = tid % PPR, prow = tid / PPR;
   const int pd = pc * 16 < a.head_dim ? pc * 16 : 0;
+  const unsigned koff = (unsigned)(prow & 31) * kss + pd, voff = (unsigned)(prow & 31) * vss + pd;
   u32x4 kraw[NP], vraw[NP];
-  Half32 h0, h1;
-  auto load_tile = [&]() {  // loads the next tile and moves on; nb is even
-    h0 = half(page_a, nb_in, nb);
-    int in1 = nb_in + 1, idx1 = nb_idx;
-    if (in1 >= a.page_blocks) {
-      in1 = 0;
-      ++idx1;
+  auto step_block = [&](int& idx, int& in) {
+    if (++in >= page_blocks) {
+      in = 0;
+      ++idx;
     }
-    if (nb + 1 <= last_block) h1 = half(page_b, in1, nb + 1);
-    else h1 = h0;  // no key there: copies of rows that exist
+  };
+  auto load_entries = [&]() {
+    int i1 = nb_idx, in = nb_in;
+    step_block(i1, in);
+    in_flight0 = tbl[min(nb_idx, last_entry) + zero];
+    in_flight1 = tbl[min(i1, last_entry) + zero];
+  };
+  auto load_tile = [&]() {
+    int idx1 = nb_idx, in1 = nb_in;
+    step_block(idx1, in1);
+    int left0 = Lk - 1 - nb * 32, left1 = left0 - 32;
+    unsigned p0 = (unsigned)page0, p1 = (unsigned)page1;
+    unsigned r0 = (unsigned)nb_in, r1 = (unsigned)in1;
     nb += 2;
     nb_idx = idx1;
-    nb_in = in1 + 1;
-    if (nb_in >= a.page_blocks) {
-      nb_in = 0;
-      ++nb_idx;
+    nb_in = in1;
+    step_block(nb_idx, nb_in);
+    load_entries();
+    if (left1 < 0) {  // no key in the second half: copies of rows that exist
+      left1 = left0;
+      p1 = p0;
+      r1 = r0;
     }
+    next_hid0 = p0 >= num_pages;
+    next_hid1 = p1 >= num_pages;
+    p0 = next_hid0 ? 0u : p0;
+    p1 = next_hid1 ? 0u : p1;
+    const unsigned char* k0 = kh + (uint64_t)p0 * k_sp + (uint64_t)(r0 * 32u) * kss;
+    const unsigned char* k1 = kh + (uint64_t)p1 * k_sp + (uint64_t)(r1 * 32u) * kss;
+    const unsigned char* v0 = vh + (uint64_t)p0 * v_sp + (uint64_t)(r0 * 32u) * vss;
+    const unsigned char* v1 = vh + (uint64_t)p1 * v_sp + (uint64_t)(r1 * 32u) * vss;
+    const bool full = left1 >= 31;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const bool second = __builtin_amdgcn_readfirstlane(prow + RPP * i) >= 32;
-      const unsigned char* kb = second ? h1.k : h0.k;
-      const unsigned char* vb = second ? h1.v : h0.v;
-      const unsigned row = (unsigned)min((prow + RPP * i) & 31, second ? h1.left : h0.left);
-      kraw[i] = *(const u32x4*)(kb + row * kss + pd);
-      vraw[i] = *(const u32x4*)(vb + row * vss + pd);
+      const bool second = RPP == 64 ? wave >= 2 : RPP * i >= 32;
+      const unsigned char* kb = second ? k1 : k0;
+      const unsigned char* vb = second ? v1 : v0;
+      constexpr unsigned down = RPP == 16 ? 16 : 0;  // (16 rows a pass: odd passes are the lower half of their 32)
+      if (full) {
+        kraw[i] = *(const u32x4*)(kb + (uint64_t)((i & 1) * down) * kss + koff);
+        vraw[i] = *(const u32x4*)(vb + (uint64_t)((i & 1) * down) * vss + voff);
+      } else {  // the sequence's last tile: rows clamped to its last one
+        const unsigned row = (unsigned)min((prow + RPP * i) & 31, second ? left1 : left0);
+        kraw[i] = *(const u32x4*)(kb + row * kss + pd);
+        vraw[i] = *(const u32x4*)(vb + row * vss + pd);
+      }
     }
+    const unsigned b0 = (unsigned)(((uint64_t)r0 * scale_inv) >> 31), b1 = (unsigned)(((uint64_t)r1 * scale_inv) >> 31);
+    nk0 = ksp[(uint64_t)p0 * ks_sp + (uint64_t)b0 * ks_sb + zero];
+    nk1 = ksp[(uint64_t)p1 * ks_sp + (uint64_t)b1 * ks_sb + zero];
+    nv0 = vsp[(uint64_t)p0 * vs_sp + (uint64_t)b0 * vs_sb + zero];
+    nv1 = vsp[(uint64_t)p1 * vs_sp + (uint64_t)b1 * vs_sb + zero];
+  };
+  auto uniform = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); };
+  auto arrived = [&]() {  // what was in flight becomes the current tile's, and the next one's entries
+    page0 = __builtin_amdgcn_readfirstlane(in_flight0);
+    page1 = __builtin_amdgcn_readfirstlane(in_flight1);
+    hid0 = next_hid0;
+    hid1 = next_hid1;
+    sk0 = uniform(nk0);
+    sk1 = uniform(nk1);
+    sv0 = hid0 ? 0.f : uniform(nv0);
+    sv1 = hid1 ? 0.f : uniform(nv1);
   };
   int st_k[NP], st_v[NP];  // LDS offsets of this thread's pieces (the second chunk is at ^ 16)
 #pragma unroll
@@ -528,10 +569,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
                  Stored<T, F>::template pair<1>(w1)};
   };
   auto store_tile = [&](int buf) {
+    if (next_hid0 || next_hid1) {  // what was loaded in their place may be NaN, and must not meet a probability of 0
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const bool second = RPP == 64 ? wave >= 2 : RPP * i >= 32;
+        if (second ? next_hid1 : next_hid0) vraw[i] = u32x4{0, 0, 0, 0};
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const bool second = __builtin_amdgcn_readfirstlane(prow + RPP * i) >= 32;
-      if (second ? h1.hidden : h0.hidden) vraw[i] = u32x4{0, 0, 0, 0};  // may be NaN, and must not meet a probability of 0
       unsigned char* base = smem + buf * TILE;
       *(u32x4*)(base + st_k[i]) = convert(kraw[i][0], kraw[i][1]);
       *(u32x4*)(base + (st_k[i] ^ 16)) = convert(kraw[i][2], kraw[i][3]);
@@ -541,8 +587,10 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   };
 
   if (ntiles > jt0) {
-    seek(jt0);
-    request();
+    load_entries();
+    page0 = __builtin_amdgcn_readfirstlane(in_flight0);
+    page1 = __builtin_amdgcn_readfirstlane(in_flight1);
+    load_tile();
   }
 
   // ---- Q through the K and V buffers: 64 rows in each pair of them, whole rows an instruction ----
@@ -595,20 +643,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
   float m_run = -INFINITY, base_run = 0.f, l_run = 0.f;
-  float ref = 1.17549435e-38f;  // O is held in units of the largest V scale so far
+  float ref = 1.17549435e-38f, ref_inv = 0.f;  // O is held in units of the largest V scale so far
 
   auto tile = [&](int j, auto bufc) {
     constexpr int BUF = decltype(bufc)::value;
     __syncthreads();  // tile j is in LDS; everyone is done with the other buffer
     const bool more = j + 1 < ntiles;
     // scores are in units of c0 and c1 per 32 keys; scale 0 (and a K scale of 0) must not meet the -inf of a masked score
-    const float c0 = fmaxf(a.scale_log2 * h0.ks, 1e-30f), c1 = fmaxf(a.scale_log2 * h1.ks, 1e-30f);
-    const float vs0 = h0.vs, vs1 = h1.vs;
-    const bool hid0 = h0.hidden, hid1 = h1.hidden;
-    if (more) {
-      load_tile();
-      if (j + 2 < ntiles) request();
-    }
+    const float c0 = fmaxf(a.scale_log2 * sk0, 1e-30f), c1 = fmaxf(a.scale_log2 * sk1, 1e-30f);
+    if (more) load_tile();
     if (wave_live && j * BN <= wave_hi) {
       f32x16 s0, s1;
 #pragma unroll
@@ -670,21 +713,22 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[i][v] *= f;
       }
-      const float top = fmaxf(vs0, vs1);
+      const float top = fmaxf(sv0, sv1);
       if (top > ref) {  // workgroup-uniform and rare
         const float f = ref / top;
         ref = top;
+        ref_inv = kLazyLift<T> / ref;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[i][v] *= f;
       }
       // The V scale of 32 keys enters as an addend of their exponents, and is divided out of their sum again: two
-      // instructions instead of one for each probability.  A scale that is 0 or next to it becomes 2^-60 of the largest,
-      // where it cannot be seen.
-      const float vf0 = fmaxf(vs0 / ref, 8.67361738e-19f), vf1 = fmaxf(vs1 / ref, 8.67361738e-19f);
-      const float b0 = base_run - __builtin_amdgcn_logf(vf0 * kLazyLift<T>), b1 = base_run - __builtin_amdgcn_logf(vf1 * kLazyLift<T>);
-      const float u0 = 1.f / (vf0 * kLazyLift<T>), u1 = 1.f / (vf1 * kLazyLift<T>);
+      // instructions instead of one for each probability.  A scale that is 0 or next to it becomes 2^-60 of the largest
+      // (or 2^-67), where it cannot be seen.
+      const float vf0 = fmaxf(sv0 * ref_inv, 8.67361738e-19f), vf1 = fmaxf(sv1 * ref_inv, 8.67361738e-19f);
+      const float b0 = base_run - __builtin_amdgcn_logf(vf0), b1 = base_run - __builtin_amdgcn_logf(vf1);
+      const float u0 = __builtin_amdgcn_rcpf(vf0), u1 = __builtin_amdgcn_rcpf(vf1);
 
       auto vfrag = [&](int mb, int t) {
         const s16x4 lo = lds_read_tr_lds(vptr[mb] + BUF * TILE + (16 * t) * ROWB);
@@ -716,13 +760,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
       }
       l_run += rs[0] * u0 + rs[1] * u1;
     }
-    if (more) store_tile(BUF ^ 1);
+    if (more) {
+      store_tile(BUF ^ 1);
+      arrived();
+    }
   };
 
   if (ntiles > jt0) {
-    load_tile();
-    if (jt0 + 1 < ntiles) request();
     store_tile(0);
+    arrived();
     int j = jt0;
     for (; j + 1 < ntiles; j += 2) {
       tile(j, IC<0>{});
@@ -732,21 +778,22 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   }
 
   // ---- epilogue ----
+  const ArgsPtr e = args_again();
   l_run = pair_sum32(l_run);
   const float o_unit = ref / kLazyLift<T>;
-  if (a.n_splits > 1) {
+  if (e->n_splits > 1) {
     if (r < R) {
-      const int64_t slot = (((int64_t)b * a.heads_q + hk * a.group + hg) * a.seqlen_q + qr) * a.n_splits + split;
-      float* dst = a.ws_o + slot * a.head_dim;
+      const int64_t slot = (((int64_t)b * e->heads_q + hk * e->group + hg) * e->seqlen_q + qr) * e->n_splits + split;
+      float* dst = e->ws_o + slot * e->head_dim;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int v4 = 0; v4 < 4; ++v4) {
           const int d = 32 * mb + 8 * v4 + 4 * g;
-          if (d < a.head_dim)
+          if (d < e->head_dim)
             *(f32x4*)(dst + d) = f32x4{o[mb][4 * v4] * o_unit, o[mb][4 * v4 + 1] * o_unit, o[mb][4 * v4 + 2] * o_unit, o[mb][4 * v4 + 3] * o_unit};
         }
-      if (g == 0) *(f32x2*)(a.ws_ml + slot * 2) = f32x2{m_run, l_run};
+      if (g == 0) *(f32x2*)(e->ws_ml + slot * 2) = f32x2{m_run, l_run};
     }
     return;
   }
@@ -763,18 +810,18 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
           u32x2{Mma<T>::pack2(o[mb][4 * v4] * inv, o[mb][4 * v4 + 1] * inv), Mma<T>::pack2(o[mb][4 * v4 + 2] * inv, o[mb][4 * v4 + 3] * inv)};
   constexpr int RPS = 64 / CPR;
   const int sr = lane / CPR, sch = lane % CPR;
-  unsigned char* ob = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)rows.first * a.o_ss + (int64_t)hk * a.group * a.o_sh;
+  unsigned char* ob = e->out + (e->cu_q ? 0 : (int64_t)b * e->o_sb) + (int64_t)rows.first * e->o_ss + (int64_t)hk * e->group * e->o_sh;
 #pragma unroll
   for (int i = 0; i < 32 / RPS; ++i) {
     const int rl = i * RPS + sr, rr = m0 + 32 * wave + rl;
     const u32x4 x = *(const u32x4*)(stage + rl * OSTR + sch * 16);
-    if (rr < R && sch * 8 < a.head_dim) {
-      const int rq = rr / a.group, rh = rr - rq * a.group;
-      *(u32x4*)(ob + (int64_t)rq * a.o_ss + (int64_t)rh * a.o_sh + sch * 16) = x;
+    if (rr < R && sch * 8 < e->head_dim) {
+      const int rq = rr / e->group, rh = rr - rq * e->group;
+      *(u32x4*)(ob + (int64_t)rq * e->o_ss + (int64_t)rh * e->o_sh + sch * 16) = x;
     }
   }
   if (r < R && g == 0)
-    a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)(hk * a.group + hg) * a.lse_sh + (int64_t)(rows.first + qr) * a.lse_ss] =
+    e->lse[(e->cu_q ? 0 : (int64_t)b * e->lse_sb) + (int64_t)(hk * e->group + hg) * e->lse_sh + (int64_t)(rows.first + qr) * e->lse_ss] =
         l_run != 0.f ? (m_run + __builtin_log2f(l_run)) * kLn2 : INFINITY;
 }
 
@@ -895,7 +942,7 @@ int fa_kv_attn_launch(const fa_kv_attn_params* p, void* workspace, size_t worksp
   a.num_pages = p->num_pages; a.table_pages = p->table_pages; a.page_size = p->page_size;
   a.page_blocks = p->page_size / 32;
   const uint64_t sb = (uint64_t)p->scale_block / 32;  // exact: a page has at most 2^15 blocks
-  a.scale_inv = ((1ULL << 32) + sb - 1) / sb;
+  a.scale_inv = (uint32_t)(((1ULL << 31) + sb - 1) / sb);
   a.is_causal = p->is_causal; a.neg_scale = p->scale < 0.f ? 1 : 0;
   a.n_splits = plan.splits; a.row_blocks = plan.row_blocks;
   a.scale_log2 = fabsf(p->scale) * kLog2e;

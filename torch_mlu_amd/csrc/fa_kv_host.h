@@ -56,6 +56,9 @@ inline int pool_validate(const P* p) {
   if (p->dtype != FA_DTYPE_FP16 && p->dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
   if (p->format != FA_KV_E4M3 && p->format != FA_KV_INT8) return FA_ERR_UNSUPPORTED;
   if (p->kp_stride_s > kMaxRowStride || p->vp_stride_s > kMaxRowStride) return FA_ERR_UNSUPPORTED;
+  if (p->kp_stride_p > 0x7fffffffLL || p->vp_stride_p > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
+  for (int i = 0; i < 6; ++i)
+    if (scales[i] > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
   return FA_OK;
 }
 
