@@ -38,9 +38,11 @@ struct AArgs {
   int32_t num_pages, table_pages, page_size;
   int32_t page_blocks;      // 32-row blocks of a page
   uint32_t scale_inv;       // ceil(2^31 / n) for scale blocks of n 32-row blocks: (block in the page * scale_inv) >> 31 is its scale
-  int32_t is_causal, neg_scale, n_splits, row_blocks;
+  int32_t is_causal, neg_scale, n_splits;
+  int32_t row_blocks;       // of a sequence; packed calls on the tile kernel: places for the blocks of all sequences
   float scale_log2;
-  float* ws_o;   // [batch * heads_q * seqlen_q * n_splits][head_dim]
+  int64_t rows_q;  // query rows of all sequences
+  float* ws_o;   // [query rows of all sequences][heads_q][n_splits][head_dim]
   float* ws_ml;  // [...][2]: maximum (log2 domain), sum
 };
 
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
           a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(rows.first + qr) * a.lse_ss] =
               sum != 0.f ? (M + __builtin_log2f(sum)) * kLn2 : INFINITY;
       } else {
-        const int64_t slot = (((int64_t)b * a.heads_q + h) * a.seqlen_q + qr) * a.n_splits + split;
+        const int64_t slot = ((rows.place + qr) * a.heads_q + h) * a.n_splits + split;
         if (d < a.head_dim) *(f32x4*)(a.ws_o + slot * a.head_dim + d) = acc;
         if (d == 0) *(f32x2*)(a.ws_ml + slot * 2) = f32x2{M, sum};
       }
@@ -431,17 +433,48 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, c32 = lane & 31;
 
-  const unsigned turn = (blockIdx.x >> 3) / (unsigned)a.row_blocks;  // as in fa_kv_attn_kernel
-  const unsigned unit = turn * 8 + (blockIdx.x & 7);
-  const int rb = a.row_blocks - 1 - (int)((blockIdx.x >> 3) - turn * a.row_blocks);
-  const unsigned bhk = unit / (unsigned)a.n_splits;
-  const int split = (int)(unit - bhk * a.n_splits);
-  const int b = (int)(bhk / (unsigned)a.heads_k), hk = (int)(bhk - (unsigned)b * a.heads_k);
-  if (b >= a.batch) return;
+  int b, hk, split, rb;
+  if (a.cu_q) {
+    // The sequences' blocks of 128 rows share the grid without a place for blocks that a shorter one has not (a workgroup that
+    // exits takes its LDS for a microsecond or two, and the ones behind it wait): with c rows before it, sequence b begins at
+    // place c * group / 128 + b, which leaves room for its blocks and at most one place too many.
+    const unsigned nhs = (unsigned)(a.heads_k * a.n_splits);
+    unsigned hs, place;
+    if (nhs % 8 == 0) {  // a head's blocks one after the other on one XCD
+      const unsigned grp = (blockIdx.x >> 3) / (unsigned)a.row_blocks;
+      place = (blockIdx.x >> 3) - grp * (unsigned)a.row_blocks;
+      hs = grp * 8 + (blockIdx.x & 7);
+    } else {
+      place = blockIdx.x / nhs;
+      hs = blockIdx.x - place * nhs;
+    }
+    ConstI32Ptr cu = (ConstI32Ptr)(uintptr_t)a.cu_q;
+    auto begin = [&](int i) { return (unsigned)((uint64_t)min(max(cu[i], 0), a.total_q) * (unsigned)a.group / BM) + (unsigned)i; };
+    int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before this place
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (begin(mid) <= place) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    rb = (int)(place - begin(lo));
+    hk = (int)(hs / (unsigned)a.n_splits);
+    split = (int)(hs - (unsigned)hk * a.n_splits);
+  } else {
+    const unsigned turn = (blockIdx.x >> 3) / (unsigned)a.row_blocks;  // as in fa_kv_attn_kernel
+    const unsigned unit = turn * 8 + (blockIdx.x & 7);
+    const unsigned bhk = unit / (unsigned)a.n_splits;
+    rb = (int)((blockIdx.x >> 3) - turn * a.row_blocks);
+    split = (int)(unit - bhk * a.n_splits);
+    b = (int)(bhk / (unsigned)a.heads_k);
+    hk = (int)(bhk - (unsigned)b * a.heads_k);
+    if (b >= a.batch) return;
+  }
 
   const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
-  const int R = rows.count * a.group, m0 = rb * BM;
-  if (m0 >= R) return;
+  const int R = rows.count * a.group, blocks = (R + BM - 1) / BM;
+  if ((unsigned)rb >= (unsigned)blocks) return;
+  const int m0 = (blocks - 1 - rb) * BM;  // the one with the most keys first
   const int Lk = min(max(a.used[b], 0), a.table_pages * a.page_size);
   const int shift = a.is_causal ? Lk - rows.aligned : 0x3fffffff;
   const int last_q = (min(m0 + BM, R) - 1) / a.group;
@@ -783,7 +816,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   const float o_unit = ref / kLazyLift<T>;
   if (e->n_splits > 1) {
     if (r < R) {
-      const int64_t slot = (((int64_t)b * e->heads_q + hk * e->group + hg) * e->seqlen_q + qr) * e->n_splits + split;
+      const int64_t slot = ((rows.place + qr) * e->heads_q + hk * e->group + hg) * e->n_splits + split;
       float* dst = e->ws_o + slot * e->head_dim;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
@@ -829,12 +862,28 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
 template <typename T>
 __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (r >= (int64_t)a.batch * a.heads_q * a.seqlen_q) return;
-  const int qr = (int)(r % a.seqlen_q), bh = (int)(r / a.seqlen_q);
-  const int h = bh % a.heads_q, b = bh / a.heads_q;
-  const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
-  if (qr >= rows.count) return;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (query row, head)
+  if (r >= a.rows_q * a.heads_q) return;
+  const int64_t t = r / a.heads_q;
+  const int h = (int)(r - t * a.heads_q);
+  int b, qr, first = 0;
+  if (a.cu_q) {
+    ConstI32Ptr cu = (ConstI32Ptr)(uintptr_t)a.cu_q;
+    int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before this row
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cu[mid] <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
+    first = rows.first;
+    qr = (int)t - first;
+    if (qr < 0 || qr >= rows.count) return;
+  } else {
+    b = (int)(t / a.seqlen_q);
+    qr = (int)(t - (int64_t)b * a.seqlen_q);
+  }
   const int D = a.head_dim, ns = a.n_splits;
   const float* po = a.ws_o + r * ns * D;
   f32x2 v = {-INFINITY, 0.f};
@@ -859,11 +908,11 @@ __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
     for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o);
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   if (sub == 0 && d < D) {
-    unsigned char* p = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(rows.first + qr) * a.o_ss + (int64_t)h * a.o_sh + d * 2;
+    unsigned char* p = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(first + qr) * a.o_ss + (int64_t)h * a.o_sh + d * 2;
     *(u32x2*)p = u32x2{Mma<T>::pack2(acc[0] * inv, acc[1] * inv), Mma<T>::pack2(acc[2] * inv, acc[3] * inv)};
   }
   if (lane == 0)
-    a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(rows.first + qr) * a.lse_ss] =
+    a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(first + qr) * a.lse_ss] =
         sum != 0.f ? (M + __builtin_log2f(sum)) * kLn2 : INFINITY;
 }
 
@@ -871,10 +920,12 @@ __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
 using namespace fa::kvhost;
 
 int64_t grid_of(const AArgs& a) { return ((int64_t)a.batch * a.heads_k * a.n_splits + 7) / 8 * 8 * a.row_blocks; }
+int64_t packed_grid_of(const AArgs& a) { return (int64_t)a.heads_k * a.n_splits * a.row_blocks; }
 
 template <typename T>
 int launch_merge(const AArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.batch * a.heads_q * a.seqlen_q;
+  const int64_t rows = a.rows_q * a.heads_q;
+  if (rows > 0x7fffffffLL * 4) return FA_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((fa_kv_merge_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
@@ -894,7 +945,7 @@ int launch_tile(const AArgs& a, hipStream_t st) {
   constexpr int lds = 4 * 64 * DP * 2;
   constexpr auto kfn = fa_kv_tile_kernel<T, F, DP>;
   if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
-  const int64_t n = grid_of(a);
+  const int64_t n = a.cu_q ? packed_grid_of(a) : grid_of(a);
   if (n > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(kfn, dim3((unsigned)n), dim3(256), lds, st, a);
   if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
@@ -947,7 +998,8 @@ int fa_kv_attn_launch(const fa_kv_attn_params* p, void* workspace, size_t worksp
   a.n_splits = plan.splits; a.row_blocks = plan.row_blocks;
   a.scale_log2 = fabsf(p->scale) * kLog2e;
   a.ws_o = (float*)workspace;
-  a.ws_ml = a.ws_o + (need ? (size_t)p->batch * p->heads_q * p->seqlen_q * plan.splits * p->head_dim : 0);
+  a.rows_q = attn_rows(p);
+  a.ws_ml = a.ws_o + (need ? (size_t)a.rows_q * p->heads_q * plan.splits * p->head_dim : 0);
   hipStream_t st = (hipStream_t)stream;
   if (p->dtype == FA_DTYPE_BF16)
     return p->format == FA_KV_E4M3 ? launch_attn<__bf16, FA_KV_E4M3>(a, plan.tiles, st) : launch_attn<__bf16, FA_KV_INT8>(a, plan.tiles, st);

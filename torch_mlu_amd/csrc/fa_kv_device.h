@@ -39,12 +39,13 @@ struct Stored<T, FA_KV_INT8> {
 // sequence b's query rows: first row and how many, clipped to what exists and to the longest the caller named
 struct QRows {
   int first, count, aligned;  // aligned: the true length, which the causal mask goes by
+  int64_t place;              // of its first row among those of all sequences
 };
 __device__ __forceinline__ QRows query_rows(const int32_t* cu, int b, int seqlen_q, int total_q) {
-  if (!cu) return QRows{0, seqlen_q, seqlen_q};
+  if (!cu) return QRows{0, seqlen_q, seqlen_q, (int64_t)b * seqlen_q};
   const int first = min(max(cu[b], 0), total_q);
   const int n = min(max(cu[b + 1], first), total_q) - first;
-  return QRows{first, min(n, seqlen_q), n};
+  return QRows{first, min(n, seqlen_q), n, first};
 }
 
 }  // namespace fa

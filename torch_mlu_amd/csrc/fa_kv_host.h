@@ -100,9 +100,32 @@ inline int attn_validate(const fa_kv_attn_params* p) {
 // How the call is cut: 16 * tiles (query row, head of the group) pairs a workgroup, `splits` slices of the key range.
 struct AttnPlan {
   int32_t tiles;      // 1, 2 or 4 tiles of 16 rows: the streaming kernel; 8: the tile kernel
-  int32_t row_blocks; // workgroups that share a (sequence, kv head, slice)
+  int32_t row_blocks; // workgroups that share a (sequence, kv head, slice); packed, tile kernel: those of all sequences
   int32_t splits;
 };
+// Slices of the tile kernel: two workgroups share a CU (one at head_dim 256), and one that has it to itself takes two thirds of
+// the time; a start and an end cost about 5 tiles, the join of the slices 2 and its partial results' bytes, of which 11 MB pass
+// while a tile is computed.  Measured (us, bf16, 32 / 8 heads, head_dim 128, e4m3; in the chosen number of slices, in one, in the
+// nearest others): 500 rows over 32768 keys 324 in 4 (829; 399 in 3, 344 in 6), 4 x 512 over 4096 168 in 1 (178 in 2), packed
+// prompts and decodes 16 x 512 over 4096 198 in 2 (206; 201 in 3), 4 x 512 over 16384 212 in 3 (423; 298 in 2, 232 in 4).
+inline int64_t tile_slices(int64_t units, int64_t tiles, int64_t rows, int head_dim) {
+  const double slots = head_dim > 128 ? 256 : 512;
+  double least = 0;
+  int64_t best = 1;
+  for (int64_t n = 1; n <= FA_MAX_SPLITS && (n == 1 || tiles >= 8 * n); ++n) {
+    const double x = (double)units * (double)n / slots, whole = floor(x), part = x - whole;
+    const double rounds = whole + (part == 0 ? 0 : (part <= 0.5 ? 0.66 : 1));
+    const double cost = rounds * ((double)tiles / (double)n + 5) + (n > 1 ? 2 + (double)rows * (double)n * (8.0 * head_dim + 16) / 11e6 : 0);
+    if (n == 1 || cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
+}
+
+// query rows of all sequences, those that no packed sequence owns among them
+inline int64_t attn_rows(const fa_kv_attn_params* p) { return p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q; }
 inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
   AttnPlan r;
   const int64_t rows = (int64_t)p->seqlen_q * (p->heads_q / p->heads_k);
@@ -111,26 +134,32 @@ inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
   if (r.row_blocks < 1) r.row_blocks = 1;
   const int64_t keys = (int64_t)p->table_pages * p->page_size;
   const int64_t blocks = r.tiles == 8 ? (keys + 63) / 64 : (keys + 31) / 32;
-  const int64_t units = (int64_t)p->batch * p->heads_k * r.row_blocks;
+  int64_t units = (int64_t)p->batch * p->heads_k * r.row_blocks;
+  if (r.tiles == 8 && p->cu_seqlens_q) {
+    // a sequence with c rows before it begins at place c * group / 128 + its number
+    const int64_t places = (int64_t)p->total_q * (p->heads_q / p->heads_k) / 128 + p->batch;
+    r.row_blocks = places > 0x7fffffff ? 0x7fffffff : (int32_t)places;
+    units = places * p->heads_k;
+  }
   int64_t n = p->num_splits;
   if (n == 0) {
     n = 1;
     if (r.tiles == 8) {
-      while (n * 2 <= FA_MAX_SPLITS && units * n * 2 <= 512 && blocks / (n * 2) >= 16) n *= 2;
+      n = tile_slices(units, blocks, attn_rows(p) * p->heads_q, p->head_dim);
     } else {
       while (n * 2 <= FA_MAX_SPLITS && units * n * 2 <= 1024 && keys / (n * 2) >= 256) n *= 2;
     }
   }
   if (n > blocks) n = blocks > 0 ? blocks : 1;
   // partial sums within 1 GiB
-  const int64_t slots = (int64_t)p->batch * p->heads_k * rows;
+  const int64_t slots = attn_rows(p) * p->heads_q;
   while (n > 1 && slots > (1LL << 30) / (n * (p->head_dim * 4 + 8))) n /= 2;
   r.splits = (int32_t)n;
   return r;
 }
 inline size_t attn_workspace_bytes(const fa_kv_attn_params* p, const AttnPlan& r) {
   if (r.splits <= 1) return 0;
-  return (size_t)p->batch * p->heads_q * p->seqlen_q * r.splits * ((size_t)p->head_dim * 4 + 8);
+  return (size_t)attn_rows(p) * p->heads_q * r.splits * ((size_t)p->head_dim * 4 + 8);
 }
 
 inline int rope_validate(const fa_rope_params* p) {
