@@ -8,7 +8,7 @@
  * Exported by libfa_kv.so.  The rules are those of fa_fwd.h: plain C, all pointers are device pointers, no allocation, no
  * synchronisation, no exception crosses; work is enqueued on the caller's stream; FA_OK or a negative code, nothing is
  * enqueued on an error.  The *_validate functions make the host checks alone and touch no GPU.  Strides between pages and those
- * of scales are below 2^31, strides between a page's rows at most 2^25.  What stands on the device
+ * of scales are below 2^31, strides between a page's rows below 2^24.  What stands on the device
  * (lengths, tables, slots) cannot be refused: each call says what a bad value does; none reads or writes out of bounds.
  * No counterpart in the reference, whose attention ops take whole tensors of 16-bit values.
  */

@@ -39,7 +39,8 @@ struct AArgs {
   int32_t page_blocks;      // 32-row blocks of a page
   uint32_t scale_inv;       // ceil(2^31 / n) for scale blocks of n 32-row blocks: (block in the page * scale_inv) >> 31 is its scale
   int32_t is_causal, neg_scale, n_splits;
-  int32_t row_blocks;       // of a sequence; packed calls on the tile kernel: places for the blocks of all sequences
+  int32_t hw_log2;          // streaming kernel: log2 of the heads of a workgroup
+  int32_t row_blocks;       // tile kernel: of a sequence; packed calls: places for the blocks of all sequences
   float scale_log2;
   int64_t rows_q;  // query rows of all sequences
   float* ws_o;   // [query rows of all sequences][heads_q][n_splits][head_dim]
@@ -59,16 +60,19 @@ template <>
 constexpr float kLazyLift<_Float16> = 128.0f;
 
 // A wavefront streams 32-key blocks straight into registers, in the layouts that v_mfma_f32_16x16x32 wants:
-//   S^T (keys x rows) = K Q^T: lane (L, G) = (lane & 15, lane >> 4) holds key L's bytes 64 c + 16 G ... + 15, which are the
-//     contraction's elements of two steps; Q is laid out to match, as the order of a contraction is free.
+//   S^T (keys x rows) = K Q^T: lane (L, G) = (lane & 15, lane >> 4) holds DP / 4 bytes of key L from DP / 4 * G on, which are
+//     its part of every step of the contraction; Q is laid out to match, as the order of a contraction is free.
 //   O^T (d x rows) = V^T P^T: lane (L, G) holds bytes VB L ... VB L + VB - 1 of the 8 keys 4 G + j and 16 + 4 G + j, j < 4,
 //     which are the keys of its own scores, so P needs no exchange; byte i of a lane goes to the product that makes rows
 //     d = VB L + i, and two keys' bytes are put side by side before they are converted.
-// So K and V pass through no LDS, every byte is read once in whole cache lines, and the four wavefronts of a workgroup, which
-// take turns in the key blocks, meet only at the end.
-template <typename T, int F, int DP, int CT>
-__global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP <= 128 ? 2 : 1)) fa_kv_attn_kernel(const AArgs a) {
-  constexpr int NW = 4;
+// So K and V pass through no LDS, and a wavefront's next blocks are on their way while it computes.
+//
+// A row of a token and head has only 128 bytes at head_dim 128, and memory is read at its full rate only where neighbours
+// are read together (64 sequences of 8192 keys, 8 kv heads: 204 us a head a workgroup, 182 with one kv head in the cache): half
+// of a workgroup's wavefronts take the neighbouring head of the same blocks.  Those of one head take turns in the blocks, and
+// meet in LDS at the end.
+template <typename T, int F, int DP, int CT, int NW>
+__global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (CT <= 2 && DP <= 128 ? 2 : 1)) fa_kv_attn_kernel(const AArgs a) {
   constexpr int KC = DP / 64;  // 16-byte pieces of a key a lane holds
   constexpr int KS = DP / 32;  // steps of the contraction over head_dim
   constexpr int VB = DP / 16;  // bytes of a key of V a lane holds = 16-row blocks of O^T
@@ -78,44 +82,45 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int L = lane & 15, G = lane >> 4;
+  const int hw = 1 << a.hw_log2, turns = NW >> a.hw_log2, turn = wave >> a.hw_log2;
 
-  // consecutive workgroups go round the 8 XCDs: those that share K and V (the row blocks of one sequence, head and slice) are
-  // neighbours on one, and a sequence's heads, whose lengths are the same, are spread over all
-  const unsigned turn = (blockIdx.x >> 3) / (unsigned)a.row_blocks;
-  const unsigned unit = turn * 8 + (blockIdx.x & 7);
-  const int rb = a.row_blocks - 1 - (int)((blockIdx.x >> 3) - turn * a.row_blocks);
-  const unsigned bhk = unit / (unsigned)a.n_splits;
-  const int split = (int)(unit - bhk * a.n_splits);
-  const int b = (int)(bhk / (unsigned)a.heads_k), hk = (int)(bhk - (unsigned)b * a.heads_k);
-  if (b >= a.batch) return;  // the grid has a multiple of 8 units
+  const unsigned groups = (unsigned)a.heads_k >> a.hw_log2;
+  const unsigned unit = blockIdx.x / (unsigned)a.n_splits;
+  const int split = (int)(blockIdx.x - unit * (unsigned)a.n_splits);
+  const int b = (int)(unit / groups), hk0 = (int)(unit - (unsigned)b * groups) << a.hw_log2;
+  const int hk = hk0 + (wave & (hw - 1));
 
+  // the first table entry, asked for before it is known whether the sequence has that key
+  ConstI32Ptr tbl = (ConstI32Ptr)(uintptr_t)(a.table + (int64_t)b * a.bt_stride);
+  const int blk0 = split * turns + turn, stride = a.n_splits * turns;
+  const int first_idx = blk0 / a.page_blocks, first_in = blk0 - first_idx * a.page_blocks;
+  const int first_page = first_idx < a.table_pages ? tbl[first_idx] : 0;
   const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
-  const int R = rows.count * a.group, r0 = rb * 16 * CT;
-  if (r0 >= R) return;
+  const int R = rows.count * a.group;  // at most 16 CT
+  if (R <= 0) return;
   const int Lk = min(max(a.used[b], 0), a.table_pages * a.page_size);
-  const int first_q = r0 / a.group, last_q = (min(r0 + 16 * CT, R) - 1) / a.group;
+  const int last_q = (R - 1) / a.group;
   // row i of the sequence sees keys up to shift + i
   const int shift = a.is_causal ? Lk - rows.aligned : 0x3fffffff;
-  const int mask_from = min(Lk, shift + first_q + 1);  // first key that some row does not see
+  const int mask_from = min(Lk, shift + 1);  // first key that some row does not see
   const int keys = min(Lk, max(shift + last_q + 1, 0));
 
+  // Every n-th 32-key block is this wavefront's: slices of a sequence are equally long whatever its length, and which table
+  // entry comes first does not wait for it.
   const int nblk = (keys + 31) >> 5;
-  const int per_split = (nblk + a.n_splits - 1) / a.n_splits;
-  const int blk_begin = split * per_split, blk_end = min(nblk, blk_begin + per_split);
-  const int blk0 = blk_begin + wave;
-  const int n_my = max(0, (blk_end - blk0 + NW - 1) / NW);
+  const int n_my = max(0, (nblk - blk0 + stride - 1) / stride);
 
   int lim[CT];  // the last key that this lane's row sees
   s16x8 qf[CT][KS];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int r = r0 + 16 * ct + L;
+    const int r = 16 * ct + L;
     const int qr = min(r, R - 1) / a.group, g = min(r, R - 1) - qr * a.group;
     lim[ct] = min(Lk - 1, shift + qr);
     const unsigned char* qp = a.q + (a.cu_q ? 0 : (int64_t)b * a.q_sb) + (int64_t)(rows.first + qr) * a.q_ss + (int64_t)(hk * a.group + g) * a.q_sh;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int d = 64 * (s >> 1) + 16 * G + 8 * (s & 1);
+      const int d = 16 * KC * G + 8 * s;
       u32x4 x = {0, 0, 0, 0};
       if (r < R && d < a.head_dim) x = *(const u32x4*)(qp + d * 2);
       if (a.neg_scale) x ^= 0x80008000u;
@@ -136,23 +141,18 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
   float ref = 1.17549435e-38f;
 
   if (n_my > 0) {
-    ConstI32Ptr tbl = (ConstI32Ptr)(uintptr_t)(a.table + (int64_t)b * a.bt_stride);
     const unsigned char* kh = a.k + (int64_t)hk * a.k_sh;
     const unsigned char* vh = a.v + (int64_t)hk * a.v_sh;
     ConstF32Ptr ksp = (ConstF32Ptr)(uintptr_t)(a.ks + (int64_t)hk * a.ks_sh);
     ConstF32Ptr vsp = (ConstF32Ptr)(uintptr_t)(a.vs + (int64_t)hk * a.vs_sh);
     const unsigned kss = (unsigned)a.k_ss, vss = (unsigned)a.v_ss;
+    const int stride_idx = stride / a.page_blocks, stride_in = stride - stride_idx * a.page_blocks;
     int kd[KC];
 #pragma unroll
-    for (int c = 0; c < KC; ++c) kd[c] = 64 * c + 16 * G < a.head_dim ? 64 * c + 16 * G : 0;
+    for (int c = 0; c < KC; ++c) kd[c] = 16 * (KC * G + c) < a.head_dim ? 16 * (KC * G + c) : 0;
     const int vd = VB * L < a.head_dim ? VB * L : 0;
-    const unsigned voff = 4 * G * vss + vd;
-    unsigned koff[KC];
-#pragma unroll
-    for (int c = 0; c < KC; ++c) koff[c] = L * kss + kd[c];
 
-    int pg_idx = blk0 / a.page_blocks, pg_in = blk0 - pg_idx * a.page_blocks;
-    int page = tbl[pg_idx];
+    int pg_idx = first_idx, pg_in = first_in, page = first_page;
 
     struct Block {
       const unsigned char* k;
@@ -173,8 +173,9 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
       x.ks = ksp[p * a.ks_sp + sb * a.ks_sb];
       x.vs = x.hidden ? 0.f : vsp[p * a.vs_sp + sb * a.vs_sb];
       x.left = Lk - 1 - blk * 32;
-      pg_in += NW;
-      while (pg_in >= a.page_blocks) {
+      pg_in += stride_in;
+      pg_idx += stride_idx;
+      if (pg_in >= a.page_blocks) {
         pg_in -= a.page_blocks;
         ++pg_idx;
       }
@@ -184,21 +185,21 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
 
     u32x4 kr[2][KC];
     unsigned vr[8][VW];
+    // Rows behind the sequence's last one are that one again.  Addresses are clamped in every block rather than in a branch for
+    // the last: with loads in branches the compiler cannot tell how many are on their way, and waits for too many.
     auto load_k = [&](const Block& x) {
-      if (x.left >= 31) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t) {
+        const unsigned row = __umul24((unsigned)min(16 * t + L, x.left), kss);
 #pragma unroll
-          for (int c = 0; c < KC; ++c) kr[t][c] = *(const u32x4*)(x.k + (uint64_t)(16u * t) * kss + koff[c]);
-      } else {  // the sequence's last block: rows clamped to its last one
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int c = 0; c < KC; ++c) kr[t][c] = *(const u32x4*)(x.k + (unsigned)min(16 * t + L, x.left) * kss + kd[c]);
+        for (int c = 0; c < KC; ++c) kr[t][c] = *(const u32x4*)(x.k + (row + kd[c]));
       }
+      __builtin_amdgcn_sched_barrier(0);  // loads stay in their order, for the same reason
     };
     auto load_v = [&](const Block& x) {
-      auto get = [&](int j, const unsigned char* p) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned char* p = x.v + (__umul24((unsigned)min(4 * G + (j < 4 ? j : 12 + j), x.left), vss) + vd);
         if constexpr (VW == 1) {
           vr[j][0] = *(const unsigned*)p;
         } else if constexpr (VW == 2) {
@@ -210,14 +211,8 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
 #pragma unroll
           for (int i = 0; i < 4; ++i) vr[j][i] = y[i];
         }
-      };
-      if (x.left >= 31) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) get(j, x.v + (uint64_t)(unsigned)(j < 4 ? j : 12 + j) * vss + voff);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) get(j, x.v + (unsigned)min(4 * G + (j < 4 ? j : 12 + j), x.left) * vss + vd);
       }
+      __builtin_amdgcn_sched_barrier(0);
     };
 
     auto step = [&](const Block& x, int blk, auto&& after_k, auto&& after_v) {
@@ -323,22 +318,22 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
     load_k(x);
     load_v(x);
     int blk = blk0;
-    for (int it = 0; it + 1 < n_my; ++it, blk += NW) {
-      const Block y = next_block(blk + NW, it + 2 < n_my);
+    for (int it = 0; it + 1 < n_my; ++it, blk += stride) {
+      const Block y = next_block(blk + stride, it + 2 < n_my);
       step(x, blk, [&] { load_k(y); }, [&] { load_v(y); });
       x = y;
     }
     step(x, blk, [] {}, [] {});
   }
 
-  // ---- the four wavefronts' partials, 16 rows at a time ----
+  // ---- the wavefronts' partials, 16 rows at a time ----
   constexpr int OS = DP + 4;
   float* so = (float*)smem;                        // [NW][16][OS]
   float* sml = (float*)(smem + NW * 16 * OS * 4);  // [NW][16][2]
   const float o_unit = ref / kLift<T>;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    if (r0 + 16 * ct >= R) break;
+    if (16 * ct >= R) break;
     float ls = l[ct];
     ls += __shfl_xor(ls, 16);
     ls = pair_sum32(ls);
@@ -358,27 +353,24 @@ __global__ void __launch_bounds__(256, CT == 1 && DP <= 128 ? 4 : (CT == 2 && DP
       sml[(wave * 16 + L) * 2 + 1] = ls;
     }
     __syncthreads();
-    const int nrows = min(16, R - r0 - 16 * ct);
+    const int nrows = min(16, R - 16 * ct);
     constexpr int TPR = DP / 4;
-    for (int item = tid; item < nrows * TPR; item += NW * 64) {
-      const int i = item / TPR, d = (item % TPR) * 4;
-      float mw[NW], M = -INFINITY;
-#pragma unroll
-      for (int y = 0; y < NW; ++y) {
-        mw[y] = sml[(y * 16 + i) * 2];
-        M = fmaxf(M, mw[y]);
-      }
+    for (int item = tid; item < hw * nrows * TPR; item += NW * 64) {
+      const int hi = item / TPR, d = (item % TPR) * 4;
+      const int hh = hi / nrows, i = hi - hh * nrows;
+      float M = -INFINITY;
+      for (int y = 0; y < turns; ++y) M = fmaxf(M, sml[((y * hw + hh) * 16 + i) * 2]);
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       float sum = 0.f;
-#pragma unroll
-      for (int y = 0; y < NW; ++y) {
-        const float ly = sml[(y * 16 + i) * 2 + 1];
+      for (int y = 0; y < turns; ++y) {
+        const int at = (y * hw + hh) * 16 + i;
+        const float ly = sml[at * 2 + 1];
         if (ly == 0.f) continue;  // a wavefront that saw no key of this row (a NaN goes on to the result)
-        const float f = fast_exp2(mw[y] - M);
+        const float f = fast_exp2(sml[at * 2] - M);
         sum += ly * f;
-        acc += *(const f32x4*)(so + (y * 16 + i) * OS + d) * f;
+        acc += *(const f32x4*)(so + at * OS + d) * f;
       }
-      const int r = r0 + 16 * ct + i, qr = r / a.group, h = hk * a.group + r - qr * a.group;
+      const int r = 16 * ct + i, qr = r / a.group, h = (hk0 + hh) * a.group + r - qr * a.group;
       if (a.n_splits == 1) {
         const float inv = sum != 0.f ? 1.f / sum : 0.f;
         if (d < a.head_dim) {
@@ -461,7 +453,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
     hk = (int)(hs / (unsigned)a.n_splits);
     split = (int)(hs - (unsigned)hk * a.n_splits);
   } else {
-    const unsigned turn = (blockIdx.x >> 3) / (unsigned)a.row_blocks;  // as in fa_kv_attn_kernel
+    // consecutive workgroups go round the 8 XCDs: those that share K and V (the row blocks of one sequence, head and slice) are
+    // neighbours on one, and a sequence's heads, whose lengths are the same, are spread over all
+    const unsigned turn = (blockIdx.x >> 3) / (unsigned)a.row_blocks;
     const unsigned unit = turn * 8 + (blockIdx.x & 7);
     const unsigned bhk = unit / (unsigned)a.n_splits;
     rb = (int)((blockIdx.x >> 3) - turn * a.row_blocks);
@@ -858,12 +852,31 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
         l_run != 0.f ? (m_run + __builtin_log2f(l_run)) * kLn2 : INFINITY;
 }
 
-// Joins the slices of a row: one wavefront a row, 4 elements of head_dim a lane, so that DP = 128 takes two slices at a time.
-template <typename T>
+// Joins the slices of a row (a query row and head).  WPR wavefronts work on one: 4 where rows are too few to fill the chip with
+// one each, otherwise 1.  A lane takes 4 elements of head_dim of every SPW-th slice, a load instruction 1 KiB; the loads of
+// the first slices are under way before their maxima are there, so that what is left is about one memory latency.
+template <typename T, int WPR>
 __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (query row, head)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = WPR == 4 ? wave : 0;
+  const int64_t r = WPR == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (r >= a.rows_q * a.heads_q) return;
+  const int D = a.head_dim, ns = a.n_splits;
+  const int lps = D <= 64 ? 16 : (D <= 128 ? 32 : 64), spw = 64 / lps;  // lanes a slice, slices an instruction
+  const int sub = lane / lps, d = (lane % lps) * 4;
+  const float* po = a.ws_o + r * ns * D + min(d, D - 4);
+  f32x2 v = {-INFINITY, 0.f};
+  if (lane < ns) v = *(const f32x2*)(a.ws_ml + r * ns * 2 + 2 * lane);
+  constexpr int U = 4;
+  const int s_step = WPR * spw;
+  f32x4 x[U];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = *(const f32x4*)(po + (int64_t)min(s0 + u * s_step, ns - 1) * D);
+  };
+  int s0 = wr * spw + sub;
+  load(s0);
+
   const int64_t t = r / a.heads_q;
   const int h = (int)(r - t * a.heads_q);
   int b, qr, first = 0;
@@ -879,33 +892,43 @@ __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
     const QRows rows = query_rows(a.cu_q, b, a.seqlen_q, a.total_q);
     first = rows.first;
     qr = (int)t - first;
-    if (qr < 0 || qr >= rows.count) return;
+    if (qr < 0 || qr >= rows.count) return;  // (uniform over the wavefronts of the row)
   } else {
     b = (int)(t / a.seqlen_q);
     qr = (int)(t - (int64_t)b * a.seqlen_q);
   }
-  const int D = a.head_dim, ns = a.n_splits;
-  const float* po = a.ws_o + r * ns * D;
-  f32x2 v = {-INFINITY, 0.f};
-  if (lane < ns) v = *(const f32x2*)(a.ws_ml + r * ns * 2 + 2 * lane);
+
   float M = v[0];
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-  const float f = v[1] == 0.f ? 0.f : fast_exp2(v[0] - M);
+  const float f = v[1] == 0.f ? 0.f : fast_exp2(v[0] - M);  // 0: a slice without a visible key for this row
   float sum = v[1] * f;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-  const int lps = D <= 64 ? 16 : (D <= 128 ? 32 : 64), spw = 64 / lps;
-  const int sub = lane / lps, d = (lane % lps) * 4;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < ns; s += spw) {
-    const int at = s + sub;
-    const float fs = __shfl(f, min(at, 63));
-    if (at < ns && d < D && fs > 0.f) acc += *(const f32x4*)(po + (int64_t)at * D + d) * fs;
+  for (;;) {
+    // what was loaded in the place of a slice that does not exist must not enter the sum at all, not even times 0: it may be
+    // infinite
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * s_step;
+      const float fs = __shfl(f, min(s, 63));
+      if (s < ns) acc += x[u] * fs;
+    }
+    s0 += U * s_step;
+    if (s0 - sub - wr * spw >= ns) break;  // (uniform)
+    load(s0);
   }
   for (int o = lps; o < 64; o <<= 1)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o);
+  if constexpr (WPR == 4) {
+    __shared__ f32x4 part[4][64];
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+    acc = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+  }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   if (sub == 0 && d < D) {
     unsigned char* p = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(first + qr) * a.o_ss + (int64_t)h * a.o_sh + d * 2;
@@ -926,17 +949,18 @@ template <typename T>
 int launch_merge(const AArgs& a, hipStream_t st) {
   const int64_t rows = a.rows_q * a.heads_q;
   if (rows > 0x7fffffffLL * 4) return FA_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((fa_kv_merge_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  if (rows < 2048) hipLaunchKernelGGL((fa_kv_merge_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((fa_kv_merge_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 template <typename T, int F, int DP, int CT>
 int launch_attn(const AArgs& a, hipStream_t st) {
-  constexpr int lds = 4 * 16 * ((DP + 4) * 4 + 8);
-  constexpr auto kfn = fa_kv_attn_kernel<T, F, DP, CT>;
+  constexpr int NW = stream_waves(DP, CT), lds = NW * 16 * ((DP + 4) * 4 + 8);
+  constexpr auto kfn = fa_kv_attn_kernel<T, F, DP, CT, NW>;
   if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
-  const int64_t n = grid_of(a);
+  const int64_t n = (int64_t)a.batch * (a.heads_k >> a.hw_log2) * a.n_splits;
   if (n > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(kfn, dim3((unsigned)n), dim3(256), lds, st, a);
+  hipLaunchKernelGGL(kfn, dim3((unsigned)n), dim3(NW * 64), lds, st, a);
   if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
   return a.n_splits > 1 ? launch_merge<T>(a, st) : FA_OK;
 }
@@ -995,7 +1019,7 @@ int fa_kv_attn_launch(const fa_kv_attn_params* p, void* workspace, size_t worksp
   const uint64_t sb = (uint64_t)p->scale_block / 32;  // exact: a page has at most 2^15 blocks
   a.scale_inv = (uint32_t)(((1ULL << 31) + sb - 1) / sb);
   a.is_causal = p->is_causal; a.neg_scale = p->scale < 0.f ? 1 : 0;
-  a.n_splits = plan.splits; a.row_blocks = plan.row_blocks;
+  a.n_splits = plan.splits; a.row_blocks = plan.row_blocks; a.hw_log2 = plan.hw_log2;
   a.scale_log2 = fabsf(p->scale) * kLog2e;
   a.ws_o = (float*)workspace;
   a.rows_q = attn_rows(p);

@@ -13,7 +13,7 @@
 namespace fa {
 namespace kvhost {
 
-constexpr int64_t kMaxRowStride = 1 << 25;  // bytes between the rows of a page: 32 rows stay below a 32-bit offset
+constexpr int64_t kMaxRowStride = (1 << 24) - 1;  // bytes between the rows of a page: an operand of a 24-bit product
 
 inline bool misaligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 // n strides that are not negative and multiples of `unit`
@@ -97,12 +97,18 @@ inline int attn_validate(const fa_kv_attn_params* p) {
   return FA_OK;
 }
 
-// How the call is cut: 16 * tiles (query row, head of the group) pairs a workgroup, `splits` slices of the key range.
+// How the call is cut: 16 * tiles (query row, head of the group) pairs a workgroup and head, `splits` slices of the key range.
 struct AttnPlan {
   int32_t tiles;      // 1, 2 or 4 tiles of 16 rows: the streaming kernel; 8: the tile kernel
-  int32_t row_blocks; // workgroups that share a (sequence, kv head, slice); packed, tile kernel: those of all sequences
+  int32_t hw_log2;    // streaming kernel: log2 of the neighbouring kv heads of a workgroup
+  int32_t row_blocks; // tile kernel: workgroups that share a (sequence, kv head, slice); packed: those of all sequences
   int32_t splits;
 };
+// wavefronts of the streaming kernel's workgroups, as many as the registers let a CU hold twice, at least once
+constexpr int stream_waves(int dp, int tiles) { return dp <= 128 && tiles <= 2 ? 8 : 4; }
+// query rows of all sequences, those that no packed sequence owns among them
+inline int64_t attn_rows(const fa_kv_attn_params* p) { return p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q; }
+
 // Slices of the tile kernel: two workgroups share a CU (one at head_dim 256), and one that has it to itself takes two thirds of
 // the time; a start and an end cost about 5 tiles, the join of the slices 2 and its partial results' bytes, of which 11 MB pass
 // while a tile is computed.  Measured (us, bf16, 32 / 8 heads, head_dim 128, e4m3; in the chosen number of slices, in one, in the
@@ -124,31 +130,44 @@ inline int64_t tile_slices(int64_t units, int64_t tiles, int64_t rows, int head_
   return best;
 }
 
-// query rows of all sequences, those that no packed sequence owns among them
-inline int64_t attn_rows(const fa_kv_attn_params* p) { return p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q; }
+// Slices of the streaming kernel: workgroups for every CU while a slice keeps a block for each of its turns, and beyond 4096
+// keys slices of 1024, which even out different lengths and a last round of long ones; of 4096 where every CU has a workgroup
+// anyway, as a full batch has nothing to even out (64 x 8192, lengths 15/16 ... 1: 186 in 1, 191 in 2, 200 in 8).  Measured (us, e4m3, 32 / 8 heads,
+// head_dim 128, lengths 1/4 ... 1 of the given; the chosen number of slices: time; others): 1 x 4097 32: 10.0; 16: 11.3,
+// 64: 10.3.  4 x 8192 16: 16.5; 8: 20, 32: 17.  16 x 2048 4: 15.4; 2: 19.6, 8: 16.7.  64 x 2048 1: 34.4; 2: 35.5.  16 x 16384
+// 16: 59; 4: 74, 8: 68, 32: 60.  64 x 8192 2: 149; 1: 153, 8: 142.  256 x 4096 1: 283; 2: 276.  28 / 4 heads, 128 x 4096
+// 1: 73; 2: 76.  Two neighbouring heads a workgroup against one, four and eight, each in its best number of slices: 1 x 4097
+// 10.0, 10.2, 10.4, 13.0; 64 x 8192 142, 147, 141, 141; 64 x 2048 34, 34, 37, 37; 256 x 4096 276, 291, 272, 277; 28 / 4 heads,
+// int8, 32 x 5000, two rows 32, 31, 34.
+inline int64_t stream_slices(int64_t units, int64_t turns, int64_t keys) {
+  int64_t n = (256 + units - 1) / units;
+  const int64_t most = keys / (32 * turns);
+  if (n > most) n = most;
+  if (n < 1) n = 1;
+  const int64_t longest = units >= 256 ? 4096 : 1024;
+  if (keys > 4096)
+    while (n * 2 <= FA_MAX_SPLITS && keys > longest * n && units * n < 2048) n *= 2;
+  return n < FA_MAX_SPLITS ? n : FA_MAX_SPLITS;
+}
+
 inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
   AttnPlan r;
-  const int64_t rows = (int64_t)p->seqlen_q * (p->heads_q / p->heads_k);
+  const int64_t group = p->heads_q / p->heads_k, rows = (int64_t)p->seqlen_q * group;
   r.tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 && p->head_dim <= 128 ? 4 : 8));
-  r.row_blocks = (int32_t)((rows + 16 * r.tiles - 1) / (16 * r.tiles));
-  if (r.row_blocks < 1) r.row_blocks = 1;
+  r.row_blocks = 1;
+  r.hw_log2 = 0;
   const int64_t keys = (int64_t)p->table_pages * p->page_size;
   const int64_t blocks = r.tiles == 8 ? (keys + 63) / 64 : (keys + 31) / 32;
-  int64_t units = (int64_t)p->batch * p->heads_k * r.row_blocks;
-  if (r.tiles == 8 && p->cu_seqlens_q) {
-    // a sequence with c rows before it begins at place c * group / 128 + its number
-    const int64_t places = (int64_t)p->total_q * (p->heads_q / p->heads_k) / 128 + p->batch;
-    r.row_blocks = places > 0x7fffffff ? 0x7fffffff : (int32_t)places;
-    units = places * p->heads_k;
-  }
   int64_t n = p->num_splits;
-  if (n == 0) {
-    n = 1;
-    if (r.tiles == 8) {
-      n = tile_slices(units, blocks, attn_rows(p) * p->heads_q, p->head_dim);
-    } else {
-      while (n * 2 <= FA_MAX_SPLITS && units * n * 2 <= 1024 && keys / (n * 2) >= 256) n *= 2;
-    }
+  if (r.tiles == 8) {
+    // (packed: a sequence with c rows before it begins at place c * group / 128 + its number)
+    const int64_t places = p->cu_seqlens_q ? (int64_t)p->total_q * group / 128 + p->batch : (rows + 127) / 128;
+    r.row_blocks = places > 0x7fffffff ? 0x7fffffff : (int32_t)places;
+    if (n == 0) n = tile_slices((p->cu_seqlens_q ? places : places * p->batch) * p->heads_k, blocks, attn_rows(p) * p->heads_q, p->head_dim);
+  } else {
+    const int dp = p->head_dim <= 64 ? 64 : (p->head_dim <= 128 ? 128 : 256), waves = stream_waves(dp, r.tiles);
+    r.hw_log2 = p->heads_k % 2 == 0 ? 1 : 0;
+    if (n == 0) n = stream_slices((int64_t)p->batch * (p->heads_k >> r.hw_log2), waves >> r.hw_log2, keys);
   }
   if (n > blocks) n = blocks > 0 ? blocks : 1;
   // partial sums within 1 GiB
