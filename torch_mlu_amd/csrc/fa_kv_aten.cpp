@@ -98,6 +98,16 @@ at::Tensor aligned_rows(const at::Tensor& t) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// A contiguous tensor in a part of `bytes`, which keeps the whole of it alive.  (Six small allocations cost twice the kernel.)
+at::Tensor part_of(const at::Tensor& bytes, int64_t& at_byte, at::ScalarType dtype, int64_t n) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(), c10::scalarTypeToTypeMeta(dtype));
+  const int64_t size = static_cast<int64_t>(c10::elementSize(dtype));
+  impl->set_storage_offset(at_byte / size);
+  impl->set_sizes_contiguous({n});
+  at_byte += n * size;
+  return at::Tensor(std::move(impl));
+}
+
 }  // namespace
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_plan(
@@ -116,10 +126,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   TORCH_CHECK(B <= FA_KV_MAX_BATCH, "at most ", FA_KV_MAX_BATCH, " requests, got ", B);
   TORCH_CHECK(page_size > 0, "page_size must be positive");
   TORCH_CHECK(max_tokens >= 0, "max_tokens must not be negative");
+  narrow(max_tokens, "max_tokens");
   const c10::OptionalDeviceGuard guard(dev);
-  const auto ints = cached.options();
-  at::Tensor cu = at::empty({B + 1}, ints), used = at::empty({B}, ints), positions = at::empty({max_tokens}, ints), left = at::empty({1}, ints);
-  at::Tensor slots = at::empty({max_tokens}, ints.dtype(at::kLong)), admitted = at::empty({B}, ints.dtype(at::kBool));
+  const at::Tensor bytes = at::empty({max_tokens * 12 + (2 * B + 2) * 4 + B}, cached.options().dtype(at::kByte));
+  int64_t used_bytes = 0;
+  at::Tensor slots = part_of(bytes, used_bytes, at::kLong, max_tokens), positions = part_of(bytes, used_bytes, at::kInt, max_tokens);
+  at::Tensor cu = part_of(bytes, used_bytes, at::kInt, B + 1), used = part_of(bytes, used_bytes, at::kInt, B);
+  at::Tensor left = part_of(bytes, used_bytes, at::kInt, 1), admitted = part_of(bytes, used_bytes, at::kBool, B);
   fa_kv_plan_params p{};
   p.cached = cached.data_ptr<int32_t>();
   p.new_tokens = new_tokens.data_ptr<int32_t>();

@@ -852,33 +852,37 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
         l_run != 0.f ? (m_run + __builtin_log2f(l_run)) * kLn2 : INFINITY;
 }
 
-// Joins the slices of a row (a query row and head).  WPR wavefronts work on one: 4 where rows are too few to fill the chip with
-// one each, otherwise 1.  A lane takes 4 elements of head_dim of every SPW-th slice, a load instruction 1 KiB; the loads of
-// the first slices are under way before their maxima are there, so that what is left is about one memory latency.
-template <typename T, int WPR>
+// Joins the slices of a row (a query row and head).  WPR wavefronts work on one where rows are too few to fill the chip with
+// one each; RPW rows (heads of one query row) are a wavefront's where they are many, so that the loads of all of them are under
+// way together.  A lane takes 4 elements of head_dim of every SPW-th slice, a load instruction 1 KiB; the first slices are
+// requested before their maxima are there and before it is known whose row it is: what is left is about one memory latency.
+template <typename T, int WPR, int RPW>
 __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
+  constexpr int U = RPW == 1 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = WPR == 4 ? wave : 0;
-  const int64_t r = WPR == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  if (r >= a.rows_q * a.heads_q) return;
+  const int64_t r0 = WPR == 4 ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * 4 + wave) * RPW;
+  if (r0 >= a.rows_q * a.heads_q) return;  // (RPW divides the heads)
   const int D = a.head_dim, ns = a.n_splits;
   const int lps = D <= 64 ? 16 : (D <= 128 ? 32 : 64), spw = 64 / lps;  // lanes a slice, slices an instruction
   const int sub = lane / lps, d = (lane % lps) * 4;
-  const float* po = a.ws_o + r * ns * D + min(d, D - 4);
-  f32x2 v = {-INFINITY, 0.f};
-  if (lane < ns) v = *(const f32x2*)(a.ws_ml + r * ns * 2 + 2 * lane);
-  constexpr int U = 4;
-  const int s_step = WPR * spw;
-  f32x4 x[U];
-  auto load = [&](int s0) {
+  const int s_step = WPR * spw, s_first = wr * spw + sub;
+  f32x2 v[RPW];
+  f32x4 x[RPW][U];
+  auto load = [&](int i, int s0) {
+    const float* po = a.ws_o + (r0 + i) * ns * D + min(d, D - 4);
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = *(const f32x4*)(po + (int64_t)min(s0 + u * s_step, ns - 1) * D);
+    for (int u = 0; u < U; ++u) x[i][u] = *(const f32x4*)(po + (int64_t)min(s0 + u * s_step, ns - 1) * D);
   };
-  int s0 = wr * spw + sub;
-  load(s0);
+#pragma unroll
+  for (int i = 0; i < RPW; ++i) {
+    v[i] = f32x2{-INFINITY, 0.f};
+    if (lane < ns) v[i] = *(const f32x2*)(a.ws_ml + (r0 + i) * ns * 2 + 2 * lane);
+    load(i, s_first);
+  }
 
-  const int64_t t = r / a.heads_q;
-  const int h = (int)(r - t * a.heads_q);
+  const int64_t t = r0 / a.heads_q;
+  const int h = (int)(r0 - t * a.heads_q);
   int b, qr, first = 0;
   if (a.cu_q) {
     ConstI32Ptr cu = (ConstI32Ptr)(uintptr_t)a.cu_q;
@@ -897,46 +901,47 @@ __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
     b = (int)(t / a.seqlen_q);
     qr = (int)(t - (int64_t)b * a.seqlen_q);
   }
+  unsigned char* out = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(first + qr) * a.o_ss + d * 2;
+  float* lse = a.lse + (a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)(first + qr) * a.lse_ss;
 
-  float M = v[0];
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-  const float f = v[1] == 0.f ? 0.f : fast_exp2(v[0] - M);  // 0: a slice without a visible key for this row
-  float sum = v[1] * f;
+  for (int i = 0; i < RPW; ++i) {
+    float M = v[i][0];
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (;;) {
-    // what was loaded in the place of a slice that does not exist must not enter the sum at all, not even times 0: it may be
-    // infinite
+    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    const float f = v[i][1] == 0.f ? 0.f : fast_exp2(v[i][0] - M);  // 0: a slice without a visible key for this row
+    float sum = v[i][1] * f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = s0 + u * s_step;
-      const float fs = __shfl(f, min(s, 63));
-      if (s < ns) acc += x[u] * fs;
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = s_first;;) {
+      // what was loaded in the place of a slice that does not exist must not enter the sum at all, not even times 0: it may be
+      // infinite
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + u * s_step;
+        const float fs = __shfl(f, min(s, 63));
+        if (s < ns) acc += x[i][u] * fs;
+      }
+      s0 += U * s_step;
+      if (s0 - s_first >= ns) break;  // (uniform)
+      load(i, s0);
     }
-    s0 += U * s_step;
-    if (s0 - sub - wr * spw >= ns) break;  // (uniform)
-    load(s0);
-  }
-  for (int o = lps; o < 64; o <<= 1)
+    for (int o = lps; o < 64; o <<= 1)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o);
-  if constexpr (WPR == 4) {
-    __shared__ f32x4 part[4][64];
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (wave != 0) return;
-    acc = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+      for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+    if constexpr (WPR == 4) {
+      __shared__ f32x4 part[4][64];
+      part[wave][lane] = acc;
+      __syncthreads();
+      if (wave != 0) return;
+      acc = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    }
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    if (sub == 0 && d < D)
+      *(u32x2*)(out + (int64_t)(h + i) * a.o_sh) = u32x2{Mma<T>::pack2(acc[0] * inv, acc[1] * inv), Mma<T>::pack2(acc[2] * inv, acc[3] * inv)};
+    if (lane == 0) lse[(int64_t)(h + i) * a.lse_sh] = sum != 0.f ? (M + __builtin_log2f(sum)) * kLn2 : INFINITY;
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  if (sub == 0 && d < D) {
-    unsigned char* p = a.out + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(first + qr) * a.o_ss + (int64_t)h * a.o_sh + d * 2;
-    *(u32x2*)p = u32x2{Mma<T>::pack2(acc[0] * inv, acc[1] * inv), Mma<T>::pack2(acc[2] * inv, acc[3] * inv)};
-  }
-  if (lane == 0)
-    a.lse[(a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(first + qr) * a.lse_ss] =
-        sum != 0.f ? (M + __builtin_log2f(sum)) * kLn2 : INFINITY;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -949,8 +954,11 @@ template <typename T>
 int launch_merge(const AArgs& a, hipStream_t st) {
   const int64_t rows = a.rows_q * a.heads_q;
   if (rows > 0x7fffffffLL * 4) return FA_ERR_UNSUPPORTED;
-  if (rows < 2048) hipLaunchKernelGGL((fa_kv_merge_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((fa_kv_merge_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  // four wavefronts a row until one each would give every CU two workgroups; four rows a wavefront where one each
+  // would go four rounds (in two slices 56480 rows 20 us against 28; in four 16000 rows 11 against 10)
+  if (rows < 2048) hipLaunchKernelGGL((fa_kv_merge_kernel<T, 4, 1>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  else if (rows >= 32768 && a.heads_q % 4 == 0) hipLaunchKernelGGL((fa_kv_merge_kernel<T, 1, 4>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((fa_kv_merge_kernel<T, 1, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 template <typename T, int F, int DP, int CT>

@@ -41,6 +41,7 @@ __global__ void __launch_bounds__(kPlanThreads) fa_kv_plan_kernel(const fa_kv_pl
   __shared__ int32_t s_taken;
   int32_t* s_end = lds;              // [batch] rows up to and with the request, at most max_tokens
   int32_t* s_page = lds + p.batch;   // [batch] pages given to the requests before; -1: not admitted
+  int32_t* s_cached = s_page + p.batch;
   const int tid = threadIdx.x, threads = blockDim.x;
   const int32_t free_count = min(max(*p.free_count, 0), p.free_capacity);
   const int64_t most = (int64_t)p.table_pages * p.page_size;
@@ -60,6 +61,7 @@ __global__ void __launch_bounds__(kPlanThreads) fa_kv_plan_kernel(const fa_kv_pl
     if (real) {
       s_end[b] = (int32_t)min(end, (int64_t)p.max_tokens);
       s_page[b] = in ? (int32_t)min(taken - need, (int64_t)0x7fffffff) : -1;
+      s_cached[b] = (int32_t)cached;
       if (in && need > 0) atomicMax(&s_taken, (int32_t)taken);
       if (blockIdx.x == 0) {
         if (b == 0) p.cu_seqlens[0] = 0;
@@ -88,7 +90,7 @@ __global__ void __launch_bounds__(kPlanThreads) fa_kv_plan_kernel(const fa_kv_pl
         else lo = mid + 1;
       }
       const int32_t start = lo > 0 ? s_end[lo - 1] : 0, before = s_page[lo];
-      const int32_t cached = max(p.cached[lo], 0);
+      const int32_t cached = s_cached[lo];
       pos = (int32_t)min((int64_t)cached + (t - start), (int64_t)0x7fffffff);
       if (before >= 0) {
         const uint32_t held = (uint32_t)(cached + (int64_t)p.page_size - 1) / (uint32_t)p.page_size;
@@ -135,6 +137,12 @@ struct Half<_Float16> {
   static constexpr unsigned kInf = 0x7c00;
 };
 
+// pairs of 16-bit magnitudes
+__device__ __forceinline__ unsigned max_pair(unsigned a, unsigned b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
 template <int F>
 struct Grid8;
 template <>
@@ -146,11 +154,12 @@ struct Grid8<FA_KV_E4M3> {
     e = max(e, -100);
     return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
   }
-  // four values in the format's range
+  // four values in the format's range, or NaN
   static __device__ __forceinline__ unsigned pack(const float* x) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(limit(x[0]), limit(x[1]), 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(limit(x[2]), limit(x[3]), w, true);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
   }
+  // infinities to the largest
   static __device__ __forceinline__ float limit(float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); }
   static __device__ __forceinline__ void unpack(unsigned w, float* x) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
@@ -164,15 +173,17 @@ template <>
 struct Grid8<FA_KV_INT8> {
   static __device__ __forceinline__ float needed(float amax) { return fmaxf(amax * (1.0f / 127), 7.8886091e-31f); }  // 2^-100
   static __device__ __forceinline__ unsigned pack(const float* x) {
-    unsigned w = 0;
+    // 1.5 x 2^23 + x is rounded to whole numbers, to nearest even, and has x's low byte as its own.  (The sum must not be
+    // contracted with the product that made x, which is rounded first.)
+#pragma clang fp contract(off)
+    unsigned u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // fmaxf takes its other operand for a NaN; that becomes 0
-      const float y = x[i] != x[i] ? 0.f : fminf(fmaxf(rintf(x[i]), -127.f), 127.f);
-      w |= ((unsigned)(int)y & 0xffu) << (8 * i);
-    }
-    return w;
+    for (int i = 0; i < 4; ++i) u[i] = __builtin_bit_cast(unsigned, x[i] + 12582912.0f);
+    const unsigned lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+    return lo | hi;
   }
+  // infinities to the largest, NaN to 0
+  static __device__ __forceinline__ float limit(float x) { return x != x ? 0.f : fminf(fmaxf(x, -127.f), 127.f); }
   static __device__ __forceinline__ void unpack(unsigned w, float* x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
@@ -180,10 +191,14 @@ struct Grid8<FA_KV_INT8> {
 };
 
 // A wavefront owns (a run of rows that go to one block, a head, key or value): nothing is shared, so the largest magnitude,
-// the scale and what has to be rounded again need no atomics, and the result does not depend on an order.  It goes over its
-// rows twice, once for the largest magnitude and once to store; the second time they come from the caches.
+// the scale and what has to be rounded again need no atomics, and the result does not depend on an order.  Up to 16 KiB of rows
+// (64 at head_dim 128) are loaded at once and stay in registers between the search for the largest magnitude and the
+// rounding; longer runs are read twice.  Finite values cannot leave the format's range, so only runs with an infinity or a NaN,
+// which their largest bit pattern shows, limit them.
 template <typename T, int F>
 __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
+#pragma clang fp contract(off)
+  constexpr int U = 16;
   const int lane = threadIdx.x & 63;
   const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t per_chunk = 2 * (int64_t)a.heads;
@@ -200,55 +215,87 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
   float* sh = a.scales[kv] + (int64_t)h * a.s_sh[kv];
   const int64_t x_st = a.x_st[kv], p_ss = a.p_ss[kv], p_sp = a.p_sp[kv];
 
-  auto slot_of = [&](int64_t t) -> uint32_t {  // 0xffffffff: this row goes nowhere
-    const int64_t s = a.slots[t];
-    return s >= 0 && s < (int64_t)a.n_slots ? (uint32_t)s : 0xffffffffu;
-  };
-  auto block_of = [&](uint32_t s) -> uint32_t { return s == 0xffffffffu ? s : s / a.scale_block; };
+  constexpr uint32_t kNone = 0xffffffffu;
+  auto usable = [&](int64_t s) -> uint32_t { return s >= 0 && s < (int64_t)a.n_slots ? (uint32_t)s : kNone; };  // kNone: goes nowhere
+  auto block_of = [&](uint32_t s) -> uint32_t { return s == kNone ? s : s / a.scale_block; };
 
-  // runs that begin in this chunk (at most 64 tokens)
-  const int64_t t_lane = t_begin + lane;
-  const bool inside = lane < a.chunk && t_lane < a.tokens;
-  const uint32_t b_lane = inside ? block_of(slot_of(t_lane)) : 0xffffffffu;
-  const uint32_t b_before = inside && t_lane > 0 ? block_of(slot_of(t_lane - 1)) : 0xffffffffu;
-  uint64_t begins = __ballot(b_lane != 0xffffffffu && b_lane != b_before);
+  // Lane l looks at the row l - 1 behind the chunk's first: runs that begin in the chunk (at most 32 rows), and, without a
+  // second load, how long they are, if they end within the next 31 rows.
+  const int64_t t_lane = t_begin - 1 + lane;
+  const uint32_t s_lane = t_lane >= 0 && t_lane < a.tokens ? usable(a.slots[t_lane]) : kNone;
+  const uint32_t b_lane = block_of(s_lane);
+  const uint32_t b_before = (uint32_t)__shfl_up((int)b_lane, 1);
+  uint64_t begins = __ballot(lane >= 1 && lane <= a.chunk && b_lane != kNone && b_lane != b_before);
   while (begins) {
     const int first = __builtin_ctzll(begins);
     begins &= begins - 1;
-    const int64_t t0 = t_begin + first;
+    const int64_t t0 = t_begin - 1 + first;
     const uint32_t blk = __builtin_amdgcn_readlane(b_lane, first);
     // how long the run is, and whether it has the block's first row
-    int n = 0;
-    bool fresh = false;
-    for (;;) {
-      const int64_t t = t0 + n + lane;
-      const uint32_t s = t < a.tokens ? slot_of(t) : 0xffffffffu;
-      const bool same = block_of(s) == blk;
-      const uint64_t not_same = ~__ballot(same);
-      const int k = not_same ? __builtin_ctzll(not_same) : 64;
-      fresh = fresh || __ballot(lane < k && s == blk * a.scale_block);
-      n += k;
-      if (k < 64) break;
-    }
-
-    unsigned top = 0;
-    for (int i = lr; i < n; i += RPI)
-      if (mine) {
-        const u32x4 w = *(const u32x4*)(xh + (t0 + i) * x_st);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
-          top = max(top, lo < Half<T>::kInf ? lo : 0u);
-          top = max(top, hi < Half<T>::kInf ? hi : 0u);
-        }
+    const uint64_t same = __ballot(b_lane == blk) >> first;
+    int n = ~same ? __builtin_ctzll(~same) : 64;  // (zeros come in at the top)
+    bool fresh = __ballot(s_lane == blk * a.scale_block && lane >= first && lane < first + n) != 0;
+    if (first + n == 64) {  // it may go on
+      for (;;) {
+        const int64_t t = t0 + n + lane;
+        const uint32_t s = t < a.tokens ? usable(a.slots[t]) : kNone;
+        const uint64_t other = ~__ballot(block_of(s) == blk);
+        const int k = other ? __builtin_ctzll(other) : 64;
+        fresh = fresh || __ballot(lane < k && s == blk * a.scale_block);
+        n += k;
+        if (k < 64) break;
       }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-    const float need = Grid8<F>::needed(Mma<T>::to_float((unsigned short)top));
-
+    }
     const uint32_t page = blk / a.blocks_per_page, in_page = blk - page * a.blocks_per_page;
     float* sp = sh + (int64_t)page * a.s_sp[kv] + (int64_t)in_page * a.s_sb[kv];
     const float old = fresh ? 0.f : *sp;
+
+    const int piece = U * RPI;  // rows at once
+    u32x4 x[U];
+    uint32_t at[U];
+    auto load = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u] = u32x4{0, 0, 0, 0};
+        at[u] = 0;
+        if (base + u * RPI >= n) continue;  // (uniform)
+        const int row = base + u * RPI + lr;
+        if (mine && row < n) {
+          x[u] = *(const u32x4*)(xh + (t0 + row) * x_st);
+          at[u] = (uint32_t)a.slots[t0 + row];
+        }
+      }
+    };
+    auto over_wave = [&](unsigned top) {  // the largest of all lanes' pairs
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) top = max_pair(top, (unsigned)__shfl_xor((int)top, o));
+      return max(top & 0xffffu, top >> 16);
+    };
+    unsigned top = 0;
+    for (int base = 0; base < n; base += piece) {
+      load(base);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max_pair(top, x[u][e] & 0x7fff7fffu);
+    }
+    top = over_wave(top);
+    const bool odd = top >= Half<T>::kInf;
+    if (odd) {  // once more, without what is not finite
+      top = 0;
+      for (int base = 0; base < n; base += piece) {
+        if (n > piece) load(base);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned lo = x[u][e] & 0x7fffu, hi = (x[u][e] >> 16) & 0x7fffu;
+            top = max_pair(top, (lo < Half<T>::kInf ? lo : 0u) | (hi < Half<T>::kInf ? hi << 16 : 0u));
+          }
+      }
+      top = over_wave(top);
+    }
+    const float need = Grid8<F>::needed(Mma<T>::to_float((unsigned short)top));
     const float scale = fmaxf(old, need);
     unsigned char* rows = ph + (int64_t)page * p_sp + (int64_t)(in_page * a.scale_block) * p_ss;
     if (!fresh && scale > old) {
@@ -258,11 +305,11 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
           u32x2 w = *(const u32x2*)(rows + (int64_t)i * p_ss);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x[4];
-            Grid8<F>::unpack(w[e], x);
+            float y[4];
+            Grid8<F>::unpack(w[e], y);
 #pragma unroll
-            for (int z = 0; z < 4; ++z) x[z] *= f;
-            w[e] = Grid8<F>::pack(x);
+            for (int z = 0; z < 4; ++z) y[z] = Grid8<F>::limit(y[z] * f);
+            w[e] = Grid8<F>::pack(y);
           }
           *(u32x2*)(rows + (int64_t)i * p_ss) = w;
         }
@@ -270,18 +317,25 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
     }
     if (lane == 0) *sp = scale;
     const float inv = 1.f / scale;
-    for (int i = lr; i < n; i += RPI)
-      if (mine) {
-        const u32x4 w = *(const u32x4*)(xh + (t0 + i) * x_st);
-        const uint32_t at = (uint32_t)a.slots[t0 + i] - blk * a.scale_block;
-        float x[8];
+    for (int base = 0; base < n; base += piece) {
+      if (n > piece) load(base);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (base + u * RPI >= n) break;  // (uniform)
+        float y[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[2 * e] = Mma<T>::to_float((unsigned short)(w[e] & 0xffffu)) * inv;
-          x[2 * e + 1] = Mma<T>::to_float((unsigned short)(w[e] >> 16)) * inv;
+          y[2 * e] = Mma<T>::to_float((unsigned short)(x[u][e] & 0xffffu)) * inv;
+          y[2 * e + 1] = Mma<T>::to_float((unsigned short)(x[u][e] >> 16)) * inv;
         }
-        *(u32x2*)(rows + (int64_t)at * p_ss) = u32x2{Grid8<F>::pack(x), Grid8<F>::pack(x + 4)};
+        if (odd) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = Grid8<F>::limit(y[e]);
+        }
+        if (mine && base + u * RPI + lr < n)
+          *(u32x2*)(rows + (int64_t)(at[u] - blk * a.scale_block) * p_ss) = u32x2{Grid8<F>::pack(y), Grid8<F>::pack(y + 4)};
       }
+    }
   }
 }
 
@@ -316,11 +370,13 @@ int fa_kv_plan_validate(const fa_kv_plan_params* p) { return plan_validate(p); }
 
 int fa_kv_plan_launch(const fa_kv_plan_params* p, void* stream) {
   if (const int rc = plan_validate(p)) return rc;
-  const int lds = p->batch * 8;
+  const int lds = p->batch * 12;
   constexpr auto kfn = fa_kv_plan_kernel;
-  if (!ensure_dynamic_lds<kfn>(FA_KV_MAX_BATCH * 8)) return FA_ERR_LAUNCH;
-  const int64_t wgs = ((int64_t)p->max_tokens + kPlanThreads - 1) / kPlanThreads;
-  hipLaunchKernelGGL(kfn, dim3((unsigned)(wgs < 1 ? 1 : (wgs > 256 ? 256 : wgs))), dim3(kPlanThreads), lds, (hipStream_t)stream, *p);
+  if (!ensure_dynamic_lds<kfn>(FA_KV_MAX_BATCH * 12)) return FA_ERR_LAUNCH;
+  // few requests leave most of a large workgroup idle in the scans, and its barriers cost
+  const int threads = p->batch <= 256 ? 256 : kPlanThreads;
+  const int64_t wgs = ((int64_t)p->max_tokens + threads - 1) / threads;
+  hipLaunchKernelGGL(kfn, dim3((unsigned)(wgs < 1 ? 1 : (wgs > 256 ? 256 : wgs))), dim3(threads), lds, (hipStream_t)stream, *p);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
