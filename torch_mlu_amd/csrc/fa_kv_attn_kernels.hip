@@ -499,11 +499,12 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   const unsigned ks_sb = own((unsigned)a.ks_sb), vs_sb = own((unsigned)a.vs_sb), scale_inv = own(a.scale_inv);
   const unsigned num_pages = own((unsigned)a.num_pages);
   const int page_blocks = (int)own((unsigned)a.page_blocks);
-  int zero;  // keeps the loads at wavefront-uniform addresses vector loads
+  unsigned zero;  // keeps the loads at wavefront-uniform addresses vector loads
   asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
-  const int last_block = max(Lk - 1, 0) >> 5, last_entry = last_block / page_blocks;
+  auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };  // a quotient comes from the vector unit
+  const int last_block = max(Lk - 1, 0) >> 5, last_entry = scalar(last_block / page_blocks);
   int nb = 2 * jt0;                                    // the next tile's first 32-key block,
-  int nb_idx = nb / page_blocks, nb_in = nb - nb_idx * page_blocks;  // its entry of the table and place in the page
+  int nb_idx = scalar(nb / page_blocks), nb_in = nb - nb_idx * page_blocks;  // its entry of the table and place in the page
   int page0 = 0, page1 = 0;                            // the next tile's entries
   bool hid0 = false, hid1 = false;                     // the current tile's: the entry names no page
   bool next_hid0 = false, next_hid1 = false;
@@ -513,7 +514,6 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   // loads nb's tile and the entries of the one after it
   const int pc = tid % PPR, prow = tid / PPR;
   const int pd = pc * 16 < a.head_dim ? pc * 16 : 0;
-  const unsigned koff = (unsigned)(prow & 31) * kss + pd, voff = (unsigned)(prow & 31) * vss + pd;
   u32x4 kraw[NP], vraw[NP];
   auto step_block = [&](int& idx, int& in) {
     if (++in >= page_blocks) {
@@ -524,8 +524,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   auto load_entries = [&]() {
     int i1 = nb_idx, in = nb_in;
     step_block(i1, in);
-    in_flight0 = tbl[min(nb_idx, last_entry) + zero];
-    in_flight1 = tbl[min(i1, last_entry) + zero];
+    in_flight0 = *(const int32_t*)((const unsigned char*)(tbl + min(nb_idx, last_entry)) + zero);
+    in_flight1 = *(const int32_t*)((const unsigned char*)(tbl + min(i1, last_entry)) + zero);
   };
   auto load_tile = [&]() {
     int idx1 = nb_idx, in1 = nb_in;
@@ -551,27 +551,19 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
     const unsigned char* k1 = kh + (uint64_t)p1 * k_sp + (uint64_t)(r1 * 32u) * kss;
     const unsigned char* v0 = vh + (uint64_t)p0 * v_sp + (uint64_t)(r0 * 32u) * vss;
     const unsigned char* v1 = vh + (uint64_t)p1 * v_sp + (uint64_t)(r1 * 32u) * vss;
-    const bool full = left1 >= 31;
+    // rows behind the sequence's last one are that one again
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const bool second = RPP == 64 ? wave >= 2 : RPP * i >= 32;
-      const unsigned char* kb = second ? k1 : k0;
-      const unsigned char* vb = second ? v1 : v0;
-      constexpr unsigned down = RPP == 16 ? 16 : 0;  // (16 rows a pass: odd passes are the lower half of their 32)
-      if (full) {
-        kraw[i] = *(const u32x4*)(kb + (uint64_t)((i & 1) * down) * kss + koff);
-        vraw[i] = *(const u32x4*)(vb + (uint64_t)((i & 1) * down) * vss + voff);
-      } else {  // the sequence's last tile: rows clamped to its last one
-        const unsigned row = (unsigned)min((prow + RPP * i) & 31, second ? left1 : left0);
-        kraw[i] = *(const u32x4*)(kb + row * kss + pd);
-        vraw[i] = *(const u32x4*)(vb + row * vss + pd);
-      }
+      const unsigned row = (unsigned)min((prow + RPP * i) & 31, second ? left1 : left0);
+      kraw[i] = *(const u32x4*)((second ? k1 : k0) + (__umul24(row, kss) + pd));
+      vraw[i] = *(const u32x4*)((second ? v1 : v0) + (__umul24(row, vss) + pd));
     }
     const unsigned b0 = (unsigned)(((uint64_t)r0 * scale_inv) >> 31), b1 = (unsigned)(((uint64_t)r1 * scale_inv) >> 31);
-    nk0 = ksp[(uint64_t)p0 * ks_sp + (uint64_t)b0 * ks_sb + zero];
-    nk1 = ksp[(uint64_t)p1 * ks_sp + (uint64_t)b1 * ks_sb + zero];
-    nv0 = vsp[(uint64_t)p0 * vs_sp + (uint64_t)b0 * vs_sb + zero];
-    nv1 = vsp[(uint64_t)p1 * vs_sp + (uint64_t)b1 * vs_sb + zero];
+    nk0 = *(const float*)((const unsigned char*)(ksp + ((uint64_t)p0 * ks_sp + (uint64_t)b0 * ks_sb)) + zero);
+    nk1 = *(const float*)((const unsigned char*)(ksp + ((uint64_t)p1 * ks_sp + (uint64_t)b1 * ks_sb)) + zero);
+    nv0 = *(const float*)((const unsigned char*)(vsp + ((uint64_t)p0 * vs_sp + (uint64_t)b0 * vs_sb)) + zero);
+    nv1 = *(const float*)((const unsigned char*)(vsp + ((uint64_t)p1 * vs_sp + (uint64_t)b1 * vs_sb)) + zero);
   };
   auto uniform = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); };
   auto arrived = [&]() {  // what was in flight becomes the current tile's, and the next one's entries
