@@ -119,8 +119,9 @@ FA_API int fa_kv_write_launch(const fa_kv_write_params* p, void* stream);
  * Keys of sequence b: the first seqused_k[b] (clipped to 0 ... table_pages * page_size); key r lives in page
  * block_table[b][r / page_size].  A table entry outside 0 ... num_pages - 1 hides its keys.  is_causal: query row i of Lq
  * sees key j <= Lk - Lq + i.  Rows that see no key get out = 0, lse = +inf.
- * K and V of keys beyond a sequence's end are never used, whatever bytes stand there.  A NaN of e4m3 in V reaches all rows of
- * its sequence's call that share a 32-key block with it, also those that the causal mask keeps from seeing it.
+ * K and V of keys that a row does not see, beyond a sequence's end or behind the causal mask, have no part in it, whatever
+ * bytes stand there.  A NaN (e4m3) in a key of K makes the rows that see it NaN, one in V their outputs, in that element at least
+ * and not their lse.
  */
 typedef struct fa_kv_attn_params {
   const void* q;         /* dtype elements; base and rows 16-byte aligned */

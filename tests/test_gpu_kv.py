@@ -424,6 +424,43 @@ def test_attention_large_scores():
     _check_attention(q, kp, vp, ks * 64, vs, table, lens, True)
 
 
+@pytest.mark.parametrize("Sq,heads,D", [(4, 4, 64), (4, 8, 128), (6, 16, 128), (3, 4, 256), (70, 4, 64), (200, 2, 128), (150, 2, 256)])
+@pytest.mark.parametrize("splits_keys", [300, 5000])
+def test_attention_nan_in_keys_that_some_rows_do_not_see(Sq, heads, D, splits_keys):
+    """NaN rows of K and V at some of the call's own tokens: the rows before them do not know, the rows from them on are NaN, and lse
+    of a NaN in V alone is what it is."""
+    n = splits_keys + Sq
+    kp, vp, ks, vs, table = _cache_for([n, 40 + Sq], 64, 2, D, 32, F8, 135)
+    q = _q((2, heads, Sq, D), BF, 20)
+    good, gl = tm.paged_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), table.to(DEV), ints([n, 40 + Sq]), is_causal=True, key_scales=ks.to(DEV), value_scales=vs.to(DEV))
+    first = Sq - Sq // 3 - 1  # the token, in the call, whose row is NaN
+    for which in (kp, vp):
+        bad = [t.clone() for t in (kp, vp)]
+        target = bad[0] if which is kp else bad[1]
+        pos = n - Sq + first
+        target.view(torch.uint8)[int(table[0, pos // 64]), pos % 64] = 0xff
+        out, lse = tm.paged_attention(q.to(DEV), bad[0].to(DEV), bad[1].to(DEV), table.to(DEV), ints([n, 40 + Sq]), is_causal=True, key_scales=ks.to(DEV),
+                                      value_scales=vs.to(DEV))
+        assert torch.equal(out[1], good[1]) and torch.equal(lse[1], gl[1])
+        assert torch.equal(out[0, :, :first], good[0, :, :first]) and torch.equal(lse[0, :, :first], gl[0, :, :first])
+        assert torch.isnan(out[0, :, first:]).all()
+        assert torch.isnan(lse[0, :, first:]).all() if which is kp else torch.equal(lse[0, :, first:], gl[0, :, first:])
+
+
+def test_attention_nan_in_a_query_row():
+    lens = [500, 90]
+    kp, vp, ks, vs, table = (t.to(DEV) for t in _cache_for(lens, 64, 2, 64, 32, F8, 136))
+    for Sq in (3, 40):
+        q = _q((2, 4, Sq, 64), BF, 21).to(DEV)
+        kw = dict(is_causal=True, key_scales=ks, value_scales=vs)
+        good, gl = tm.paged_attention(q, kp, vp, table, ints(lens), **kw)
+        q[0, 1, 2, 5] = math.nan
+        out, lse = tm.paged_attention(q, kp, vp, table, ints(lens), **kw)
+        assert torch.isnan(out[0, 1, 2]).all() and torch.isnan(lse[0, 1, 2])
+        out[0, 1, 2], lse[0, 1, 2] = good[0, 1, 2], gl[0, 1, 2]
+        assert torch.equal(out, good) and torch.equal(lse, gl)
+
+
 def test_attention_strided_views():
     lens, page, H, D = [200, 90], 64, 2, 64
     kp, vp, ks, vs, table = _cache_for(lens, page, H, D, 32, F8, 141)

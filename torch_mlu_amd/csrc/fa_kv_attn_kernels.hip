@@ -59,6 +59,14 @@ constexpr float kLazyLift = 1.0f;
 template <>
 constexpr float kLazyLift<_Float16> = 128.0f;
 
+// e4m3's NaN (0x7f and 0xff) among the bytes of w, which become 0; returns whether there were any.  V is searched where a mask
+// hides some of its keys: hidden ones have a probability of 0, and 0 x NaN is NaN.  A row that does see such a key is NaN.
+__device__ __forceinline__ bool take_nan(unsigned& w) {
+  const unsigned t = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x80 for each
+  w &= ~((t << 1) - (t >> 7));
+  return t != 0;
+}
+
 // A wavefront streams 32-key blocks straight into registers, in the layouts that v_mfma_f32_16x16x32 wants:
 //   S^T (keys x rows) = K Q^T: lane (L, G) = (lane & 15, lane >> 4) holds DP / 4 bytes of key L from DP / 4 * G on, which are
 //     its part of every step of the contraction; Q is laid out to match, as the order of a contraction is free.
@@ -139,6 +147,7 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (CT <= 2 &
   }
   // O is held in units of `ref`, the largest V scale so far, so that P vs / ref stays in fp16's range whatever the scales are
   float ref = 1.17549435e-38f;
+  int poison = 0;  // bit ct: this lane's row sees a NaN of V among its keys
 
   if (n_my > 0) {
     const unsigned char* kh = a.k + (int64_t)hk * a.k_sh;
@@ -245,6 +254,18 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (CT <= 2 &
             if (16 + e > lm) s[1][ct][e] = -INFINITY;
           }
         }
+        if constexpr (F == FA_KV_E4M3) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) any |= take_nan(vr[j][i]);
+            const bool bad = ((__ballot(any) >> (16 * G)) & 0xffffu) != 0;  // the 16 lanes of a G hold the same keys
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              if (bad && !x.hidden && (j < 4 ? j : 12 + j) <= lim[ct] - blk * 32 - 4 * G) poison |= 1 << ct;
+          }
+        }
       }
       if (x.vs > ref) {  // wavefront-uniform and rare
         const float f = ref / x.vs;
@@ -330,10 +351,12 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (CT <= 2 &
   constexpr int OS = DP + 4;
   float* so = (float*)smem;                        // [NW][16][OS]
   float* sml = (float*)(smem + NW * 16 * OS * 4);  // [NW][16][2]
-  const float o_unit = ref / kLift<T>;
+  poison |= __shfl_xor(poison, 16);
+  poison |= __shfl_xor(poison, 32);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     if (16 * ct >= R) break;
+    const float o_unit = (poison >> ct) & 1 ? __builtin_nanf("") : ref / kLift<T>;
     float ls = l[ct];
     ls += __shfl_xor(ls, 16);
     ls = pair_sum32(ls);
@@ -587,12 +610,31 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
     return u32x4{Stored<T, F>::template pair<0>(w0), Stored<T, F>::template pair<1>(w0), Stored<T, F>::template pair<0>(w1),
                  Stored<T, F>::template pair<1>(w1)};
   };
-  auto store_tile = [&](int buf) {
+  __shared__ int nan_key[2][BN], nan_tile[2];  // the last tile in which this key (a key) of a buffer had a NaN in V
+  if (tid < 2 * BN) (&nan_key[0][0])[tid] = -1;
+  if (tid < 2) nan_tile[tid] = -1;
+  const int shown = min(Lk - 1, shift + m0 / a.group);  // the last key that all rows of the workgroup see
+  auto store_tile = [&](int buf, int j) {
     if (next_hid0 || next_hid1) {  // what was loaded in their place may be NaN, and must not meet a probability of 0
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const bool second = RPP == 64 ? wave >= 2 : RPP * i >= 32;
         if (second ? next_hid1 : next_hid0) vraw[i] = u32x4{0, 0, 0, 0};
+      }
+    }
+    if constexpr (F == FA_KV_E4M3) {
+      if (j * BN + BN - 1 > shown) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          bool any = false;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            unsigned y = vraw[i][z];
+            any |= take_nan(y);
+            vraw[i][z] = y;
+          }
+          if (any) nan_key[buf][prow + RPP * i] = nan_tile[buf] = j;
+        }
       }
     }
 #pragma unroll
@@ -662,6 +704,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
   float m_run = -INFINITY, base_run = 0.f, l_run = 0.f;
+  bool poison = false;  // this lane's row sees a NaN of V among its keys
   float ref = 1.17549435e-38f, ref_inv = 0.f;  // O is held in units of the largest V scale so far
 
   auto tile = [&](int j, auto bufc) {
@@ -700,6 +743,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
           const int e = 8 * (v >> 2) + (v & 3);
           if (e > la) s0[v] = -INFINITY;
           if (32 + e > lb) s1[v] = -INFINITY;
+        }
+      }
+      if constexpr (F == FA_KV_E4M3) {
+        if (j * BN + BN - 1 > shown && nan_tile[BUF] == j) {
+#pragma clang loop unroll(disable)
+          for (int v = 0; v < 32; ++v) {
+            const int e = 32 * (v >> 4) + 8 * ((v & 15) >> 2) + (v & 3) + 4 * g;
+            if (nan_key[BUF][e] == j && j * BN + e <= lim_row) poison = true;
+          }
         }
       }
       // the compiler waits for the matrix pipe only in front of instructions it knows: the first read of each product is a
@@ -780,13 +832,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
       l_run += rs[0] * u0 + rs[1] * u1;
     }
     if (more) {
-      store_tile(BUF ^ 1);
+      store_tile(BUF ^ 1, j + 1);
       arrived();
     }
   };
 
   if (ntiles > jt0) {
-    store_tile(0);
+    store_tile(0, jt0);
     arrived();
     int j = jt0;
     for (; j + 1 < ntiles; j += 2) {
@@ -799,7 +851,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   // ---- epilogue ----
   const ArgsPtr e = args_again();
   l_run = pair_sum32(l_run);
-  const float o_unit = ref / kLazyLift<T>;
+  const int poison_other = __shfl_xor((int)poison, 32);
+  const float o_unit = poison || poison_other ? __builtin_nanf("") : ref / kLazyLift<T>;
   if (e->n_splits > 1) {
     if (r < R) {
       const int64_t slot = ((rows.place + qr) * e->heads_q + hk * e->group + hg) * e->n_splits + split;
