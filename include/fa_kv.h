@@ -43,7 +43,8 @@ extern "C" {
  *   slots[t]        page x page_size + offset of row t; -1 where its request is not admitted, where the page is negative and
  *                   behind the last row
  *   free_left       free_count less the pages given out: the first free_left entries of free_pages are still free
- * A free_count beyond free_capacity counts as free_capacity, one below 0 as 0.
+ * A free_count beyond free_capacity counts as free_capacity, one below 0 as 0.  Outputs overlap neither the inputs nor the
+ * table nor one another: a step's seqused becomes the next one's cached by changing places, not by being the same array.
  */
 typedef struct fa_kv_plan_params {
   const int32_t* cached;     /* [batch] */
@@ -56,7 +57,7 @@ typedef struct fa_kv_plan_params {
   int32_t* positions;        /* [max_tokens] */
   int64_t* slots;            /* [max_tokens] */
   uint8_t* admitted;         /* [batch] */
-  int32_t* free_left;        /* [1]; may not be free_count itself */
+  int32_t* free_left;        /* [1] */
   int64_t block_table_stride; /* elements */
   int32_t batch;             /* 0 ... FA_KV_MAX_BATCH */
   int32_t table_pages;       /* entries of a row, at most block_table_stride */

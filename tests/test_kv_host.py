@@ -115,6 +115,7 @@ def test_good_blocks_pass_and_null_is_refused(kind, make):
     ("fa_kv_plan", _plan, dict(batch=8193), UNS), ("fa_kv_plan", _plan, dict(page_size=0), BAD), ("fa_kv_plan", _plan, dict(table_pages=21), BAD),
     ("fa_kv_plan", _plan, dict(table_pages=1 << 20, block_table_stride=1 << 20, page_size=1 << 12), UNS),
     ("fa_kv_plan", _plan, dict(free_pages=None), BAD), ("fa_kv_plan", _plan, dict(free_left=0x5000), BAD), ("fa_kv_plan", _plan, dict(reserved=1), BAD),
+    ("fa_kv_plan", _plan, dict(seqused=0x1000), BAD), ("fa_kv_plan", _plan, dict(cu_seqlens=0x2000), BAD),
     ("fa_kv_plan", _plan, dict(max_tokens=-1), BAD), ("fa_kv_plan", _plan, dict(batch=0, cached=None, new_tokens=None, seqused=None, admitted=None), 0),
     ("fa_kv_plan", _plan, dict(free_capacity=0, free_pages=None), 0), ("fa_kv_plan", _plan, dict(max_tokens=0, slots=None, positions=None), 0),
     ("fa_kv_write", _write, dict(key=None), BAD), ("fa_kv_write", _write, dict(key=0x1008), BAD), ("fa_kv_write", _write, dict(slots=0x3004), BAD),
@@ -188,3 +189,20 @@ def test_rotary_frequencies():
     for bad in ((), (0,), (2, -1)):
         with pytest.raises(ValueError):
             torch_mlu_amd.rotary_frequencies(bad)
+
+
+def test_host_half_is_clean_under_asan_and_ubsan():
+    """Validation, plans and workspace sizes (csrc/fa_kv_host.h) over ordinary, extreme and malformed blocks, built with the address and
+    undefined-behaviour sanitizers: any overflow or out-of-bounds access ends the driver."""
+    import shutil
+
+    if shutil.which("g++") is None:
+        pytest.skip("no host C++ compiler")
+    with tempfile.TemporaryDirectory() as d:
+        exe = os.path.join(d, "kv_host_sanitize")
+        subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-static-libasan", "-fno-sanitize-recover=all", "-Wall", "-Werror",
+                        "-I" + INC, "-I" + os.path.join(ROOT, "torch_mlu_amd", "csrc"), os.path.join(ROOT, "tests", "kv_host_sanitize.cpp"), "-o", exe],
+                       check=True)
+        res = subprocess.run([exe], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr[-2000:]
+    assert re.match(r"\d+ blocks, \d+ plans", res.stdout)

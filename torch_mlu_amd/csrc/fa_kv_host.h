@@ -29,7 +29,7 @@ inline int plan_validate(const fa_kv_plan_params* p) {
   if (p->block_table_stride < p->table_pages) return FA_ERR_BAD_ARG;
   if (p->batch > FA_KV_MAX_BATCH) return FA_ERR_UNSUPPORTED;
   if ((int64_t)p->table_pages * p->page_size > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
-  if (!p->free_count || !p->cu_seqlens || !p->free_left || p->free_count == p->free_left) return FA_ERR_BAD_ARG;
+  if (!p->free_count || !p->cu_seqlens || !p->free_left) return FA_ERR_BAD_ARG;
   if (p->batch > 0 && (!p->cached || !p->new_tokens || !p->seqused || !p->admitted || (!p->block_table && p->table_pages > 0))) return FA_ERR_BAD_ARG;
   if (p->max_tokens > 0 && (!p->positions || !p->slots)) return FA_ERR_BAD_ARG;
   if (p->free_capacity > 0 && !p->free_pages) return FA_ERR_BAD_ARG;
@@ -37,6 +37,12 @@ inline int plan_validate(const fa_kv_plan_params* p) {
   for (const void* w : words)
     if (misaligned(w, 4)) return FA_ERR_BAD_ARG;
   if (misaligned(p->slots, 8)) return FA_ERR_BAD_ARG;
+  // workgroups read lengths and the count while others already write
+  const void* in[] = {p->cached, p->new_tokens, p->free_count, p->free_pages, p->block_table};
+  const void* out[] = {p->cu_seqlens, p->seqused, p->positions, p->slots, p->admitted, p->free_left};
+  for (const void* i : in)
+    for (const void* o : out)
+      if (i && i == o) return FA_ERR_BAD_ARG;
   return FA_OK;
 }
 
