@@ -52,7 +52,7 @@ int main() {
                     must(r.splits == 1 || r.splits <= (keys + 31) / 32, "no more slices than blocks");
                     must(r.tiles == 8 || rows <= 16 * r.tiles, "the streaming kernel's rows");
                     must(r.tiles == 8 || p.heads_k % (1 << r.hw_log2) == 0, "whole groups of heads");
-                    must(r.tiles == 8 || (1 << r.hw_log2) <= stream_waves(d <= 128 ? 128 : 256, r.tiles), "a wavefront a head");
+                    must(r.tiles == 8 || (1 << r.hw_log2) <= stream_waves(d <= 128 ? 128 : 256), "a wavefront a head");
                     if (r.tiles == 8 && !packed) must((int64_t)r.row_blocks * 128 >= rows, "a place for every block of rows");
                     must(attn_workspace_bytes(&p, r) == (r.splits == 1 ? 0 : (size_t)attn_rows(&p) * p.heads_q * r.splits * (d * 4 + 8)), "the workspace");
                   }

