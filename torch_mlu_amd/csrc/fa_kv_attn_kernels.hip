@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (DP <= 128
       float ks, vs;
     };
     // this wavefront's next block; the table entry of the one after it is requested
-    auto next_block = [&](int blk, bool more) -> Block {
+    auto next_block = [&](int blk, bool more) __attribute__((always_inline)) -> Block {
       Block x;
       x.hidden = (unsigned)page >= (unsigned)a.num_pages;
       const int64_t p = x.hidden ? 0 : page;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (DP <= 128
     unsigned vr[8][VW];
     // Rows behind the sequence's last one are that one again.  Addresses are clamped in every block rather than in a branch for
     // the last: with loads in branches the compiler cannot tell how many are on their way, and waits for too many.
-    auto load_k = [&](const Block& x) {
+    auto load_k = [&](const Block& x) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const unsigned row = __umul24((unsigned)min(16 * t + L, x.left), kss);
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (DP <= 128
       }
       __builtin_amdgcn_sched_barrier(0);  // loads stay in their order, for the same reason
     };
-    auto load_v = [&](const Block& x) {
+    auto load_v = [&](const Block& x) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const unsigned char* p = x.v + (__umul24((unsigned)min(4 * G + (j < 4 ? j : 12 + j), x.left), vss) + vd);
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(NW * 64, CT == 1 && DP <= 128 ? 4 : (DP <= 128
       __builtin_amdgcn_sched_barrier(0);
     };
 
-    auto step = [&](const Block& x, int blk, auto&& after_k, auto&& after_v) {
+    auto step = [&](const Block& x, int blk, auto&& after_k, auto&& after_v) __attribute__((always_inline)) {
       f32x4 s[2][CT];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -542,6 +542,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   float nk0 = 0.f, nk1 = 0.f, nv0 = 0.f, nv1 = 0.f;    // the next tile's, in flight
   int in_flight0 = 0, in_flight1 = 0;                  // entries of the tile after that, in flight
   // loads nb's tile and the entries of the one after it
+  // (The lambdas that touch register arrays are inlined by force: where one stays a call, as store_tile did for int8 at 256, the
+  // arrays live in memory: 16/1 heads of 256, 2x4 rows over 3386 keys 87 us instead of 25.)
   const int pc = tid % PPR, prow = tid / PPR;
   const int pd = pc * 16 < a.head_dim ? pc * 16 : 0;
   u32x4 kraw[NP], vraw[NP];
@@ -551,13 +553,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
       ++idx;
     }
   };
-  auto load_entries = [&]() {
+  auto load_entries = [&]() __attribute__((always_inline)) {
     int i1 = nb_idx, in = nb_in;
     step_block(i1, in);
     in_flight0 = *(const int32_t*)((const unsigned char*)(tbl + min(nb_idx, last_entry)) + zero);
     in_flight1 = *(const int32_t*)((const unsigned char*)(tbl + min(i1, last_entry)) + zero);
   };
-  auto load_tile = [&]() {
+  auto load_tile = [&]() __attribute__((always_inline)) {
     int idx1 = nb_idx, in1 = nb_in;
     step_block(idx1, in1);
     int left0 = Lk - 1 - nb * 32, left1 = left0 - 32;
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
     nv1 = *(const float*)((const unsigned char*)(vsp + ((uint64_t)p1 * vs_sp + (uint64_t)b1 * vs_sb)) + zero);
   };
   auto uniform = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); };
-  auto arrived = [&]() {  // what was in flight becomes the current tile's, and the next one's entries
+  auto arrived = [&]() __attribute__((always_inline)) {  // what was in flight becomes the current tile's, and the next one's entries
     page0 = __builtin_amdgcn_readfirstlane(in_flight0);
     page1 = __builtin_amdgcn_readfirstlane(in_flight1);
     hid0 = next_hid0;
@@ -621,7 +623,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   if (tid < 2 * BN) (&nan_key[0][0])[tid] = -1;
   if (tid < 2) nan_tile[tid] = -1;
   const int shown = min(Lk - 1, shift + m0 / a.group);  // the last key that all rows of the workgroup see
-  auto store_tile = [&](int buf, int j) {
+  auto store_tile = [&](int buf, int j) __attribute__((always_inline)) {
     if (next_hid0 || next_hid1) {  // what was loaded in their place may be NaN, and must not meet a probability of 0
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -714,7 +716,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   bool poison = false;  // this lane's row sees a NaN of V among its keys
   float ref = 1.17549435e-38f, ref_inv = 0.f;  // O is held in units of the largest V scale so far
 
-  auto tile = [&](int j, auto bufc) {
+  auto tile = [&](int j, auto bufc) __attribute__((always_inline)) {
     constexpr int BUF = decltype(bufc)::value;
     __syncthreads();  // tile j is in LDS; everyone is done with the other buffer
     const bool more = j + 1 < ntiles;
