@@ -462,10 +462,10 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
     // place c * group / 128 + b, which leaves room for its blocks and at most one place too many.
     const unsigned nhs = (unsigned)(a.heads_k * a.n_splits);
     unsigned hs, place;
-    if (nhs % 8 == 0) {  // a head's blocks one after the other on one XCD
-      const unsigned grp = (blockIdx.x >> 3) / (unsigned)a.row_blocks;
-      place = (blockIdx.x >> 3) - grp * (unsigned)a.row_blocks;
-      hs = grp * 8 + (blockIdx.x & 7);
+    if (nhs % 8 == 0) {  // a head's blocks on one XCD, one place of all its heads and slices after the other (head by head the
+                         // last slice's long blocks began when the rest was done: 16 x 512 over 4096, 194 us instead of 181)
+      place = (blockIdx.x >> 3) / (nhs >> 3);
+      hs = ((blockIdx.x >> 3) - place * (nhs >> 3)) * 8 + (blockIdx.x & 7);
     } else {
       place = blockIdx.x / nhs;
       hs = blockIdx.x - place * nhs;
