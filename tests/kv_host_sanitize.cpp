@@ -55,6 +55,8 @@ int main() {
                     must(r.tiles == 8 || (1 << r.hw_log2) <= stream_waves(d <= 128 ? 128 : 256), "a wavefront a head");
                     if (r.tiles == 8 && !packed) must((int64_t)r.row_blocks * 128 >= rows, "a place for every block of rows");
                     must(attn_workspace_bytes(&p, r) == (r.splits == 1 ? 0 : (size_t)attn_rows(&p) * p.heads_q * r.splits * (d * 4 + 8)), "the workspace");
+                    const int64_t wgs = attn_wgs(&p, r), threads = r.tiles == 8 ? 256 : 512;
+                    must(wgs >= -1 && (wgs < 0 || wgs * threads <= 0xffffffffLL), "a launch's threads in 32 bits");
                   }
   // packed: sequence b's blocks begin at place c * group / 128 + b (c: rows before it) and end before the next one's
   for (int64_t group : {1, 3, 4, 7, 16, 128})

@@ -147,6 +147,26 @@ def test_validation(kind, make, over, rc):
             assert L.fa_kv_attn_workspace_bytes(ctypes.byref(p)) == 0
 
 
+@pytest.mark.parametrize("kind,make,over,rc", [
+    # a launch has fewer than 2^32 threads: 4 runs of up to 32 rows, or 1 to 16 tokens, a workgroup of 256
+    ("fa_kv_write", _write, dict(tokens=(1 << 29) - 64), 0), ("fa_kv_write", _write, dict(tokens=1 << 29), UNS),
+    ("fa_rope", _rope, dict(batch=1, seqlen=(1 << 24) - 1, q=0x1002), 0), ("fa_rope", _rope, dict(batch=1, seqlen=1 << 24, q=0x1002), UNS),
+    ("fa_rope", _rope, dict(batch=1, seqlen=1 << 24, heads_q=1, heads_k=0), 0), ("fa_rope", _rope, dict(batch=1, seqlen=1 << 28, heads_q=1, heads_k=0), UNS),
+])
+def test_calls_beyond_one_launch_are_refused(kind, make, over, rc):
+    L, p = capi_kv.lib(), make(**over)
+    assert getattr(L, kind + "_validate")(ctypes.byref(p)) == rc
+    if rc:
+        assert getattr(L, kind + "_launch")(ctypes.byref(p), None) == rc
+
+
+@pytest.mark.parametrize("over", [dict(batch=1 << 25, num_splits=1), dict(batch=1 << 20, seqlen_q=1 << 10, num_splits=1),
+                                  dict(cu_seqlens_q=0x6000, total_q=1 << 30, seqlen_q=1 << 20, num_splits=1)])
+def test_attention_beyond_one_launch_is_refused(over):
+    p = _attn(**over)  # refused before it touches a device
+    assert capi_kv.lib().fa_kv_attn_launch(ctypes.byref(p), None, 0, None) == UNS
+
+
 def test_attention_workspace():
     """Partial results (an fp32 row, its maximum and sum) of every query row and slice; short workspaces are refused."""
     L = capi_kv.lib()

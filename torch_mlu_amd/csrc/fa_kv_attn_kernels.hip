@@ -1001,13 +1001,9 @@ __global__ void __launch_bounds__(256) fa_kv_merge_kernel(const AArgs a) {
 // ---- host ---------------------------------------------------------------------------------------------------------------
 using namespace fa::kvhost;
 
-int64_t grid_of(const AArgs& a) { return ((int64_t)a.batch * a.heads_k * a.n_splits + 7) / 8 * 8 * a.row_blocks; }
-int64_t packed_grid_of(const AArgs& a) { return (int64_t)a.heads_k * a.n_splits * a.row_blocks; }
-
 template <typename T>
 int launch_merge(const AArgs& a, hipStream_t st) {
-  const int64_t rows = a.rows_q * a.heads_q;
-  if (rows > 0x7fffffffLL * 4) return FA_ERR_UNSUPPORTED;
+  const int64_t rows = a.rows_q * a.heads_q;  // few enough for a grid, as their partial results fit the workspace
   // four wavefronts a row until one each would give every CU two workgroups; four rows a wavefront where one each
   // would go four rounds (in two slices 56480 rows 20 us against 28; in four 16000 rows 11 against 10)
   if (rows < 2048) hipLaunchKernelGGL((fa_kv_merge_kernel<T, 4, 1>), dim3((unsigned)rows), dim3(256), 0, st, a);
@@ -1016,33 +1012,29 @@ int launch_merge(const AArgs& a, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 template <typename T, int F, int DP, int CT>
-int launch_attn(const AArgs& a, hipStream_t st) {
+int launch_attn(const AArgs& a, int64_t wgs, hipStream_t st) {
   constexpr int NW = stream_waves(DP), lds = NW * 16 * ((DP + 4) * 4 + 8);
   constexpr auto kfn = fa_kv_attn_kernel<T, F, DP, CT, NW>;
   if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
-  const int64_t n = (int64_t)a.batch * (a.heads_k >> a.hw_log2) * a.n_splits;
-  if (n > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(kfn, dim3((unsigned)n), dim3(NW * 64), lds, st, a);
+  hipLaunchKernelGGL(kfn, dim3((unsigned)wgs), dim3(NW * 64), lds, st, a);
   if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
   return a.n_splits > 1 ? launch_merge<T>(a, st) : FA_OK;
 }
 template <typename T, int F, int DP>
-int launch_tile(const AArgs& a, hipStream_t st) {
+int launch_tile(const AArgs& a, int64_t wgs, hipStream_t st) {
   constexpr int lds = 4 * 64 * DP * 2;
   constexpr auto kfn = fa_kv_tile_kernel<T, F, DP>;
   if (!ensure_dynamic_lds<kfn>(lds)) return FA_ERR_LAUNCH;
-  const int64_t n = a.cu_q ? packed_grid_of(a) : grid_of(a);
-  if (n > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(kfn, dim3((unsigned)n), dim3(256), lds, st, a);
+  hipLaunchKernelGGL(kfn, dim3((unsigned)wgs), dim3(256), lds, st, a);
   if (hipGetLastError() != hipSuccess) return FA_ERR_LAUNCH;
   return a.n_splits > 1 ? launch_merge<T>(a, st) : FA_OK;
 }
 template <typename T, int F>
-int launch_attn(const AArgs& a, int tiles, hipStream_t st) {
-  if (tiles == 8) return a.head_dim <= 64 ? launch_tile<T, F, 64>(a, st) : (a.head_dim <= 128 ? launch_tile<T, F, 128>(a, st) : launch_tile<T, F, 256>(a, st));
-  if (a.head_dim <= 64) return tiles == 1 ? launch_attn<T, F, 64, 1>(a, st) : launch_attn<T, F, 64, 2>(a, st);
-  if (a.head_dim <= 128) return tiles == 1 ? launch_attn<T, F, 128, 1>(a, st) : launch_attn<T, F, 128, 2>(a, st);
-  return tiles == 1 ? launch_attn<T, F, 256, 1>(a, st) : launch_attn<T, F, 256, 2>(a, st);
+int launch_attn(const AArgs& a, int tiles, int64_t wgs, hipStream_t st) {
+  if (tiles == 8) return a.head_dim <= 64 ? launch_tile<T, F, 64>(a, wgs, st) : (a.head_dim <= 128 ? launch_tile<T, F, 128>(a, wgs, st) : launch_tile<T, F, 256>(a, wgs, st));
+  if (a.head_dim <= 64) return tiles == 1 ? launch_attn<T, F, 64, 1>(a, wgs, st) : launch_attn<T, F, 64, 2>(a, wgs, st);
+  if (a.head_dim <= 128) return tiles == 1 ? launch_attn<T, F, 128, 1>(a, wgs, st) : launch_attn<T, F, 128, 2>(a, wgs, st);
+  return tiles == 1 ? launch_attn<T, F, 256, 1>(a, wgs, st) : launch_attn<T, F, 256, 2>(a, wgs, st);
 }
 
 }  // namespace
@@ -1061,6 +1053,8 @@ int fa_kv_attn_launch(const fa_kv_attn_params* p, void* workspace, size_t worksp
   const size_t need = attn_workspace_bytes(p, plan);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return FA_ERR_BAD_ARG;
   if (p->seqlen_q == 0 || (p->cu_seqlens_q && p->total_q == 0)) return FA_OK;
+  const int64_t wgs = attn_wgs(p, plan);
+  if (wgs < 0) return FA_ERR_UNSUPPORTED;
   AArgs a;
   a.q = (const unsigned char*)p->q; a.k = (const unsigned char*)p->key_pages; a.v = (const unsigned char*)p->value_pages;
   a.ks = p->key_scales; a.vs = p->value_scales;
@@ -1088,8 +1082,8 @@ int fa_kv_attn_launch(const fa_kv_attn_params* p, void* workspace, size_t worksp
   a.ws_ml = a.ws_o + (need ? (size_t)a.rows_q * p->heads_q * plan.splits * p->head_dim : 0);
   hipStream_t st = (hipStream_t)stream;
   if (p->dtype == FA_DTYPE_BF16)
-    return p->format == FA_KV_E4M3 ? launch_attn<__bf16, FA_KV_E4M3>(a, plan.tiles, st) : launch_attn<__bf16, FA_KV_INT8>(a, plan.tiles, st);
-  return p->format == FA_KV_E4M3 ? launch_attn<_Float16, FA_KV_E4M3>(a, plan.tiles, st) : launch_attn<_Float16, FA_KV_INT8>(a, plan.tiles, st);
+    return p->format == FA_KV_E4M3 ? launch_attn<__bf16, FA_KV_E4M3>(a, plan.tiles, wgs, st) : launch_attn<__bf16, FA_KV_INT8>(a, plan.tiles, wgs, st);
+  return p->format == FA_KV_E4M3 ? launch_attn<_Float16, FA_KV_E4M3>(a, plan.tiles, wgs, st) : launch_attn<_Float16, FA_KV_INT8>(a, plan.tiles, wgs, st);
 }
 
 }  // extern "C"

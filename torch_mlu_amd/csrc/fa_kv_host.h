@@ -15,6 +15,9 @@ namespace kvhost {
 
 constexpr int64_t kMaxRowStride = (1 << 24) - 1;  // bytes between the rows of a page: an operand of a 24-bit product
 
+// a launch's threads are counted in 32 bits
+inline bool grid_fits(int64_t wgs, int64_t threads) { return wgs <= 0xffffffffLL / threads; }
+
 inline bool misaligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 // n strides that are not negative and multiples of `unit`
 inline bool bad_strides(const int64_t* s, int n, int64_t unit) {
@@ -68,6 +71,10 @@ inline int pool_validate(const P* p) {
   return FA_OK;
 }
 
+// tokens whose runs a wavefront of the write kernel looks for, and the wavefronts of a call
+inline int32_t write_chunk(const fa_kv_write_params* p) { return p->tokens >= 512 ? 32 : 1; }
+inline int64_t write_units(const fa_kv_write_params* p) { return ((int64_t)p->tokens + write_chunk(p) - 1) / write_chunk(p) * 2 * p->heads; }
+
 inline int write_validate(const fa_kv_write_params* p) {
   if (!p) return FA_ERR_BAD_ARG;
   if (p->tokens < 0 || p->heads <= 0) return FA_ERR_BAD_ARG;
@@ -78,6 +85,7 @@ inline int write_validate(const fa_kv_write_params* p) {
   if (misaligned(p->key, 16) || misaligned(p->value, 16) || misaligned(p->slots, 8)) return FA_ERR_BAD_ARG;
   const int64_t st[] = {p->key_stride_t, p->key_stride_h, p->value_stride_t, p->value_stride_h};
   if (bad_strides(st, 4, 8)) return FA_ERR_BAD_ARG;
+  if (!grid_fits((write_units(p) + 3) / 4, 256)) return FA_ERR_UNSUPPORTED;
   return FA_OK;
 }
 
@@ -185,11 +193,42 @@ inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
   r.splits = (int32_t)n;
   return r;
 }
+// workgroups of the call; below 0: more than a launch can have
+inline int64_t attn_wgs(const fa_kv_attn_params* p, const AttnPlan& r) {
+  if (r.tiles != 8) {
+    const int64_t n = (int64_t)p->batch * (p->heads_k >> r.hw_log2) * r.splits;
+    return grid_fits(n, 512) ? n : -1;
+  }
+  const int64_t per_row_block = p->cu_seqlens_q ? (int64_t)p->heads_k * r.splits : ((int64_t)p->batch * p->heads_k * r.splits + 7) / 8 * 8;
+  return per_row_block <= 0xffffffffLL / 256 / r.row_blocks ? per_row_block * r.row_blocks : -1;
+}
 inline size_t attn_workspace_bytes(const fa_kv_attn_params* p, const AttnPlan& r) {
   if (r.splits <= 1) return 0;
   return (size_t)attn_rows(p) * p->heads_q * r.splits * ((size_t)p->head_dim * 4 + 8);
 }
 
+// 16-byte pieces of a head: where every row starts at one and a piece has the pairs of one side, or whole pairs
+inline bool rope_vector(const fa_rope_params* p) {
+  const int64_t n = p->dtype == FA_DTYPE_FP32 ? 4 : 8;
+  if (p->head_dim % n || (p->interleaved ? (2 * p->pairs) % n : p->pairs % n)) return false;
+  if (misaligned(p->q, 16) || misaligned(p->q_out, 16)) return false;
+  int64_t all = p->q_stride_b | p->q_stride_s | p->q_stride_h | p->qo_stride_b | p->qo_stride_s | p->qo_stride_h;
+  if (p->heads_k > 0) {
+    if (misaligned(p->k, 16) || misaligned(p->k_out, 16)) return false;
+    all |= p->k_stride_b | p->k_stride_s | p->k_stride_h | p->ko_stride_b | p->ko_stride_s | p->ko_stride_h;
+  }
+  return (all & (n - 1)) == 0;
+}
+// Tokens of a workgroup: as many as give each of its threads two pieces, while the workgroups stay four a CU (us, one token and
+// this rule: 16384 tokens of 2 + 1 heads of 64 16.3 and 6.2, of 8 + 8 of 128 28.3 and 23.4; 2000 of 32 + 8 of 128 9.5 and 9.4).
+inline int32_t rope_tokens_per_wg(const fa_rope_params* p, bool vec) {
+  const int64_t e = vec ? (p->dtype == FA_DTYPE_FP32 ? 4 : 8) : 1, tokens = (int64_t)p->batch * p->seqlen;
+  const int64_t turned = (p->interleaved && vec ? 2 * p->pairs : p->pairs) / e, copied = (p->head_dim - 2 * p->pairs) / e;
+  const int64_t pieces = (turned + copied) * ((int64_t)p->heads_q + p->heads_k);
+  int32_t n = 1;
+  while (n < 16 && n * 2 * pieces <= 512 && tokens / (n * 2) >= 1024) n *= 2;
+  return n;
+}
 inline int rope_validate(const fa_rope_params* p) {
   if (!p) return FA_ERR_BAD_ARG;
   if (p->batch < 0 || p->seqlen < 0 || p->heads_q <= 0 || p->heads_k < 0 || p->head_dim < 2 || p->pairs < 1 || p->pairs > p->head_dim / 2) return FA_ERR_BAD_ARG;
@@ -203,20 +242,10 @@ inline int rope_validate(const fa_rope_params* p) {
     if (!p->q || !p->q_out || !p->positions || (p->heads_k > 0 && (!p->k || !p->k_out))) return FA_ERR_BAD_ARG;
     if (misaligned(p->q, size) || misaligned(p->q_out, size) || misaligned(p->positions, p->positions_64 ? 8 : 4)) return FA_ERR_BAD_ARG;
     if (p->heads_k > 0 && (misaligned(p->k, size) || misaligned(p->k_out, size))) return FA_ERR_BAD_ARG;
+    const int64_t per_wg = rope_tokens_per_wg(p, rope_vector(p));
+    if (!grid_fits(((int64_t)p->batch * p->seqlen + per_wg - 1) / per_wg, 256)) return FA_ERR_UNSUPPORTED;
   }
   return FA_OK;
-}
-// 16-byte pieces of a head: where every row starts at one and a piece has the pairs of one side, or whole pairs
-inline bool rope_vector(const fa_rope_params* p) {
-  const int64_t n = p->dtype == FA_DTYPE_FP32 ? 4 : 8;
-  if (p->head_dim % n || (p->interleaved ? (2 * p->pairs) % n : p->pairs % n)) return false;
-  if (misaligned(p->q, 16) || misaligned(p->q_out, 16)) return false;
-  int64_t all = p->q_stride_b | p->q_stride_s | p->q_stride_h | p->qo_stride_b | p->qo_stride_s | p->qo_stride_h;
-  if (p->heads_k > 0) {
-    if (misaligned(p->k, 16) || misaligned(p->k_out, 16)) return false;
-    all |= p->k_stride_b | p->k_stride_s | p->k_stride_h | p->ko_stride_b | p->ko_stride_s | p->ko_stride_h;
-  }
-  return (all & (n - 1)) == 0;
 }
 
 }  // namespace kvhost

@@ -345,9 +345,7 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
 using namespace fa::kvhost;
 
 template <typename T, int F>
-int launch_write(const WArgs& a, hipStream_t st) {
-  const int64_t units = ((int64_t)a.tokens + a.chunk - 1) / a.chunk * 2 * a.heads;
-  if (units > 0x7fffffffLL * 4) return FA_ERR_UNSUPPORTED;
+int launch_write(const WArgs& a, int64_t units, hipStream_t st) {
   hipLaunchKernelGGL((fa_kv_write_kernel<T, F>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
@@ -401,10 +399,11 @@ int fa_kv_write_launch(const fa_kv_write_params* p, void* stream) {
   a.n_slots = (uint32_t)p->num_pages * (uint32_t)p->page_size;
   a.tokens = p->tokens; a.heads = p->heads; a.head_dim = p->head_dim;
   a.scale_block = (uint32_t)p->scale_block; a.blocks_per_page = (uint32_t)(p->page_size / p->scale_block);
-  a.chunk = p->tokens >= 512 ? 32 : 1;
+  a.chunk = write_chunk(p);
+  const int64_t units = write_units(p);
   hipStream_t st = (hipStream_t)stream;
-  if (p->dtype == FA_DTYPE_BF16) return p->format == FA_KV_E4M3 ? launch_write<__bf16, FA_KV_E4M3>(a, st) : launch_write<__bf16, FA_KV_INT8>(a, st);
-  return p->format == FA_KV_E4M3 ? launch_write<_Float16, FA_KV_E4M3>(a, st) : launch_write<_Float16, FA_KV_INT8>(a, st);
+  if (p->dtype == FA_DTYPE_BF16) return p->format == FA_KV_E4M3 ? launch_write<__bf16, FA_KV_E4M3>(a, units, st) : launch_write<__bf16, FA_KV_INT8>(a, units, st);
+  return p->format == FA_KV_E4M3 ? launch_write<_Float16, FA_KV_E4M3>(a, units, st) : launch_write<_Float16, FA_KV_INT8>(a, units, st);
 }
 
 }  // extern "C"

@@ -146,13 +146,7 @@ __global__ void __launch_bounds__(256) fa_rope_kernel(const RArgs a) {
 using namespace fa::kvhost;
 
 template <typename T>
-int launch_rope(RArgs& a, bool vec, hipStream_t st) {
-  // Tokens of a workgroup: as many as give each of its threads two pieces, while the workgroups stay four a CU (us, one token and
-  // this rule: 16384 tokens of 2 + 1 heads of 64 16.3 and 6.2, of 8 + 8 of 128 28.3 and 23.4; 2000 of 32 + 8 of 128 9.5 and 9.4).
-  const int e = vec ? 16 / (int)sizeof(T) : 1;
-  const int64_t pieces = ((a.interleaved && vec ? 2 * a.pairs : a.pairs) / e + (a.head_dim - 2 * a.pairs) / e) * (int64_t)(a.heads[0] + a.heads[1]);
-  a.per_wg = 1;
-  while (a.per_wg < 16 && a.per_wg * 2 * pieces <= 512 && a.tokens / (a.per_wg * 2) >= 1024) a.per_wg *= 2;
+int launch_rope(const RArgs& a, bool vec, hipStream_t st) {
   const int64_t wgs = ((int64_t)a.tokens + a.per_wg - 1) / a.per_wg;
   const int lds = a.per_wg * a.pairs * 8;
   if (vec) hipLaunchKernelGGL((fa_rope_kernel<T, true>), dim3((unsigned)wgs), dim3(256), lds, st, a);
@@ -185,6 +179,7 @@ int fa_rope_launch(const fa_rope_params* p, void* stream) {
   a.positions_64 = p->positions_64; a.freq_64 = p->inv_freq_64; a.interleaved = p->interleaved; a.inverse = p->inverse;
   hipStream_t st = (hipStream_t)stream;
   const bool vec = rope_vector(p);
+  a.per_wg = rope_tokens_per_wg(p, vec);
   if (p->dtype == FA_DTYPE_FP32) return launch_rope<float>(a, vec, st);
   return p->dtype == FA_DTYPE_BF16 ? launch_rope<__bf16>(a, vec, st) : launch_rope<_Float16>(a, vec, st);
 }
