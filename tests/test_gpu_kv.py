@@ -539,6 +539,21 @@ def test_attention_refusals():
             tm.paged_attention(**{**ok, **over})
 
 
+def test_cache_tensors_that_want_gradients_are_refused():
+    """Neither operator has a gradient, so a scale that requires one would get none without a word."""
+    kp, vp, ks, vs, table = (t.to(DEV) for t in _cache_for([64], 64, 2, 64, 64, F8, 172))
+    q, x, slot = torch.zeros(1, 4, 1, 64, dtype=BF, device=DEV), torch.zeros(1, 2, 64, dtype=BF, device=DEV), ints([0], torch.int64)
+    for i in range(2):
+        scales = [ks, vs]
+        scales[i] = scales[i].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="for inference"):
+            tm.paged_attention(q, kp, vp, table, ints([64]), key_scales=scales[0], value_scales=scales[1])
+        with pytest.raises(RuntimeError, match="for inference"):
+            tm.paged_cache_write(x, x, kp, vp, *scales, slot)
+        with torch.no_grad():
+            tm.paged_attention(q, kp, vp, table, ints([64]), key_scales=scales[0], value_scales=scales[1])
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("form,dtype", [(F8, BF), (I8, HF)])
 def test_serving_loop(form, dtype):

@@ -55,12 +55,14 @@ void fill_pool(P& p, const at::Tensor& kp, const at::Tensor& vp, const at::Tenso
     TORCH_CHECK(t.device() == dev, pname[i], " must be on ", dev, ", got ", t.device());
     TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kChar, pname[i], " must have dtype float8_e4m3fn or int8, got ",
                 t.scalar_type());
+    check_inference(t, pname[i]);
     TORCH_CHECK(t.dim() == 4, pname[i], " must be [pages, page_size, heads, head_dim]");
     TORCH_CHECK(t.size(2) == heads && t.size(3) == head_dim, pname[i], " must have ", heads, " heads of ", head_dim, ", got ", t.sizes());
     TORCH_CHECK(t.size(3) <= 1 || t.stride(3) == 1, pname[i], " must have a contiguous last dimension");
     const at::Tensor& s = *scales[i];
     TORCH_CHECK(s.device() == dev, sname[i], " must be on ", dev, ", got ", s.device());
     TORCH_CHECK(s.scalar_type() == at::kFloat, sname[i], " must have dtype float32");
+    check_inference(s, sname[i]);
     TORCH_CHECK(s.dim() == 3 && s.size(0) == t.size(0) && s.size(2) == heads, sname[i], " must be [pages, blocks, heads], got ", s.sizes());
   }
   TORCH_CHECK(kp.scalar_type() == vp.scalar_type() && kp.sizes() == vp.sizes(), "key_pages and value_pages must have the same dtype and shape");
