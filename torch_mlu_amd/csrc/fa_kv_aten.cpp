@@ -232,7 +232,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_8bit(const at::Tensor& query,
     p.cu_seqlens_q = cu_seqlens_q->data_ptr<int32_t>();
     p.total_q = narrow(q.size(0), "the number of rows");
   } else {
-    out = at::empty({B, Sq, Hq, D}, query.options()).transpose(1, 2);
+    out = at::empty_strided({B, Hq, Sq, D}, {Sq * Hq * D, D, Hq * D, 1}, query.options());  // [B, Sq, Hq, D] in memory
     lse = at::empty({B, Hq, Sq}, floats);
     p.q_stride_b = dim_stride(q, 0); p.q_stride_h = dim_stride(q, 1); p.q_stride_s = dim_stride(q, 2);
     p.o_stride_b = out.stride(0); p.o_stride_h = out.stride(1); p.o_stride_s = out.stride(2);
