@@ -161,6 +161,34 @@ def test_write_many_rows_with_padding_and_slots_outside_the_pool(form):
 
 
 @pytest.mark.parametrize("form", [F8, I8])
+@pytest.mark.parametrize("dtype,D,page,block", [(BF, 128, 128, 128), (HF, 256, 64, 64), (BF, 96, 256, 128), (HF, 64, 512, 256), (BF, 256, 512, 512), (HF, 16, 1024, 1024)])
+def test_write_blocks_longer_than_a_wavefront_holds(form, dtype, D, page, block):
+    """Whole blocks, parts of them at both ends, single rows and rows of many requests, in a call long enough for runs to be shared;
+    infinities and NaN in some rows, blocks whose scale grows and blocks that keep theirs."""
+    H, starts = 2, [(0, 700), (page - 3, 9), (5, 1), (block + 31, 300), (2 * page - 1, 1), (17, page)]
+    P = sum(-(-(c + n) // page) for c, n in starts) + 2
+    slots = _slots(starts, P, page, D + block)
+    T = len(slots)
+    slots = [-1] * 5 + slots + [-1] * 40
+    (kp, ks), (vp, vs) = _pool(P, page, H, D, block, form, 15), _pool(P, page, H, D, block, form, 16)
+    key, value = _rows(T + 45, H, D, dtype, 17), _rows(T + 45, H, D, dtype, 18)
+    key[100, 0, 3], key[101, 1, 5], key[650, 0, 0], value[720, 1, D - 1] = math.inf, math.nan, -math.inf, math.nan
+    value[800] = 0
+    _check_write(key, value, slots, kp, vp, ks, vs)
+
+
+@pytest.mark.parametrize("H,D,page,block", [(1, 16, 64, 32), (12, 16, 64, 64), (24, 16, 32, 32), (64, 16, 96, 96), (24, 64, 256, 256), (64, 64, 256, 256)])
+def test_write_long_and_single_rows_among_one_another(H, D, page, block):
+    """Runs that begin anywhere in the tokens that are looked through together, from one of them to 32, and end in others."""
+    starts = [(9, 1), (0, 500)] + [(page * i + 7 * i, 1) for i in range(1, 40)] + [(1, 257), (block - 1, 2)] + [(5 * i, 3) for i in range(20)] + [(0, 513)]
+    P = sum(-(-(c + n) // page) for c, n in starts) + 2
+    slots = _slots(starts, P, page, H)
+    slots = slots[:501] + [-1] * 33 + slots[501:]
+    (kp, ks), (vp, vs) = _pool(P, page, H, D, block, F8, 33), _pool(P, page, H, D, block, F8, 34)
+    _check_write(_rows(len(slots), H, D, BF, 35), _rows(len(slots), H, D, BF, 36), slots, kp, vp, ks, vs)
+
+
+@pytest.mark.parametrize("form", [F8, I8])
 def test_write_rows_of_a_block_in_any_order(form):
     page, block, H, D = 64, 64, 2, 64
     (kp, ks), (vp, vs) = _pool(4, page, H, D, block, form, 21), _pool(4, page, H, D, block, form, 22)

@@ -71,9 +71,26 @@ inline int pool_validate(const P* p) {
   return FA_OK;
 }
 
-// tokens whose runs a wavefront of the write kernel looks for, and the wavefronts of a call
-inline int32_t write_chunk(const fa_kv_write_params* p) { return p->tokens >= 512 ? 32 : 1; }
-inline int64_t write_units(const fa_kv_write_params* p) { return ((int64_t)p->tokens + write_chunk(p) - 1) / write_chunk(p) * 2 * p->heads; }
+// The write kernel: wavefronts that share a run of rows, the tokens whose runs they look for, workgroups of a call.
+// A wavefront's registers hold kWriteLoads x 1 KiB of rows; four share a run where whole blocks are longer (us, one and four: 2 x
+// 7143 rows of 16 heads of 96, blocks of 128 55 and 37; 3 x 4493 of 16 of 256, blocks of 64 69 and 49; 64 x 24 of 16 of 128,
+// blocks of 256 9.7 and 12.5).  Looking through tokens that begin no run costs wavefronts, several runs for one cost time: as few
+// tokens each as leave 4096 wavefronts (us, 32 tokens and this rule: 1024 x 1 of 8 heads of 128 50 and 19, 128 x 8 13.6 and 7.0,
+// 8 x 2000 19 and 19, of 8 tokens 36).
+constexpr int kWriteLoads = 16;
+inline int write_waves(const fa_kv_write_params* p) {
+  const int fits = kWriteLoads * (512 / p->head_dim);
+  return p->scale_block > fits && p->tokens > fits ? 4 : 1;
+}
+inline int32_t write_chunk(const fa_kv_write_params* p) {
+  int32_t n = 1;
+  while (n < 32 && (int64_t)p->tokens * 2 * p->heads > (int64_t)n * 4096) n *= 2;
+  return n;
+}
+inline int64_t write_wgs(const fa_kv_write_params* p) {
+  const int64_t units = ((int64_t)p->tokens + write_chunk(p) - 1) / write_chunk(p) * 2 * p->heads, per_wg = 4 / write_waves(p);
+  return (units + per_wg - 1) / per_wg;
+}
 
 inline int write_validate(const fa_kv_write_params* p) {
   if (!p) return FA_ERR_BAD_ARG;
@@ -85,7 +102,7 @@ inline int write_validate(const fa_kv_write_params* p) {
   if (misaligned(p->key, 16) || misaligned(p->value, 16) || misaligned(p->slots, 8)) return FA_ERR_BAD_ARG;
   const int64_t st[] = {p->key_stride_t, p->key_stride_h, p->value_stride_t, p->value_stride_h};
   if (bad_strides(st, 4, 8)) return FA_ERR_BAD_ARG;
-  if (!grid_fits((write_units(p) + 3) / 4, 256)) return FA_ERR_UNSUPPORTED;
+  if (!grid_fits(write_wgs(p), 256)) return FA_ERR_UNSUPPORTED;
   return FA_OK;
 }
 

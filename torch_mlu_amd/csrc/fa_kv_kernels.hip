@@ -194,15 +194,16 @@ struct Grid8<FA_KV_INT8> {
 // A wavefront owns (a run of rows that go to one block, a head, key or value): nothing is shared, so the largest magnitude,
 // the scale and what has to be rounded again need no atomics, and the result does not depend on an order.  Up to 16 KiB of rows
 // (64 at head_dim 128) are loaded at once and stay in registers between the search for the largest magnitude and the
-// rounding; longer runs are read twice.  Finite values cannot leave the format's range, so only runs with an infinity or a NaN,
-// which their largest bit pattern shows, limit them.  12000 rows of 8 heads, head_dim 128, bf16 to e4m3: 19.4 us, 3.9 TB/s read and
-// written (27 when the rows were read twice); 64 rows: 5 us, three dependent reads.
-template <typename T, int F>
+// rounding; where blocks may be longer, a workgroup's four wavefronts (W) share those runs that are, and only runs of more than 64
+// KiB are read twice.  Finite values cannot leave the format's range, so only runs with an infinity or a NaN, which their largest
+// bit pattern shows, limit them.  12000 rows of 8 heads, head_dim 128, bf16 to e4m3: 19 us, 3.9 TB/s read and written (27 when the
+// rows were read twice); 64 rows: 5 us, three dependent reads.
+template <typename T, int F, int W>
 __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
 #pragma clang fp contract(off)
-  constexpr int U = 16;
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int U = kvhost::kWriteLoads;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t unit = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const int64_t per_chunk = 2 * (int64_t)a.heads;
   const int64_t c = unit / per_chunk;
   const int hk = (int)(unit - c * per_chunk), kv = hk >= a.heads ? 1 : 0, h = hk - kv * a.heads;
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
   const uint32_t b_lane = block_of(s_lane);
   const uint32_t b_before = (uint32_t)__shfl_up((int)b_lane, 1);
   uint64_t begins = __ballot(lane >= 1 && lane <= a.chunk && b_lane != kNone && b_lane != b_before);
+  int turn = 0;
   while (begins) {
     const int first = __builtin_ctzll(begins);
     begins &= begins - 1;
@@ -248,11 +250,15 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
         if (k < 64) break;
       }
     }
+    // Long runs are shared by the workgroup's wavefronts, which all look at the same ones; those that fit one wavefront go round.
+    const bool shared = W > 1 && n > U * RPI;
+    if (W > 1 && !shared && (turn++ & (W - 1)) != wave) continue;
+    const int rw = shared ? W : 1, wr = shared ? wave : 0;  // wavefronts of the run, this one among them
     const uint32_t page = blk / a.blocks_per_page, in_page = blk - page * a.blocks_per_page;
     float* sp = sh + (int64_t)page * a.s_sp[kv] + (int64_t)in_page * a.s_sb[kv];
-    const float old = fresh ? 0.f : *sp;
+    float old = !fresh && wr == 0 ? *sp : 0.f;  // (the one that also writes it)
 
-    const int piece = U * RPI;  // rows at once
+    const int piece = U * RPI * rw;  // rows at once
     u32x4 x[U];
     uint32_t at[U];
     auto load = [&](int base) {
@@ -260,18 +266,30 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
       for (int u = 0; u < U; ++u) {
         x[u] = u32x4{0, 0, 0, 0};
         at[u] = 0;
-        if (base + u * RPI >= n) continue;  // (uniform)
-        const int row = base + u * RPI + lr;
+        if (base + (u * rw + wr) * RPI >= n) continue;  // (uniform)
+        const int row = base + (u * rw + wr) * RPI + lr;
         if (mine && row < n) {
           x[u] = *(const u32x4*)(xh + (t0 + row) * x_st);
           at[u] = (uint32_t)a.slots[t0 + row];
         }
       }
     };
-    auto over_wave = [&](unsigned top) {  // the largest of all lanes' pairs
+    auto over_run = [&](unsigned x) {  // the largest of all lanes' pairs
 #pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) top = max_pair(top, (unsigned)__shfl_xor((int)top, o));
-      return max(top & 0xffffu, top >> 16);
+      for (int o = 32; o >= 1; o >>= 1) x = max_pair(x, (unsigned)__shfl_xor((int)x, o));
+      x = max(x & 0xffffu, x >> 16);
+      if constexpr (W > 1) if (shared) {
+        __shared__ unsigned tops[W];
+        __shared__ float before;
+        __syncthreads();  // the last exchange's readers are done
+        if (lane == 0) tops[wave] = x;
+        if (threadIdx.x == 0) before = old;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) x = max(x, tops[w]);
+        old = before;
+      }
+      return x;
     };
     unsigned top = 0;
     for (int base = 0; base < n; base += piece) {
@@ -281,7 +299,7 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = max_pair(top, x[u][e] & 0x7fff7fffu);
     }
-    top = over_wave(top);
+    top = over_run(top);
     const bool odd = top >= Half<T>::kInf;
     if (odd) {  // once more, without what is not finite
       top = 0;
@@ -295,14 +313,14 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
             top = max_pair(top, (lo < Half<T>::kInf ? lo : 0u) | (hi < Half<T>::kInf ? hi << 16 : 0u));
           }
       }
-      top = over_wave(top);
+      top = over_run(top);
     }
     const float need = Grid8<F>::needed(Mma<T>::to_float((unsigned short)top));
     const float scale = fmaxf(old, need);
     unsigned char* rows = ph + (int64_t)page * p_sp + (int64_t)(in_page * a.scale_block) * p_ss;
     if (!fresh && scale > old) {
       const float f = old / scale;
-      for (uint32_t i = lr; i < a.scale_block; i += RPI)
+      for (uint32_t i = wr * RPI + lr; i < a.scale_block; i += rw * RPI)
         if (mine) {
           u32x2 w = *(const u32x2*)(rows + (int64_t)i * p_ss);
 #pragma unroll
@@ -316,14 +334,15 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
           *(u32x2*)(rows + (int64_t)i * p_ss) = w;
         }
       WAIT_VMCNT(0);  // the rows of this call, which come next, go on top of these stores
+      if constexpr (W > 1) if (shared) __syncthreads();
     }
-    if (lane == 0) *sp = scale;
+    if (lane == 0 && wr == 0) *sp = scale;
     const float inv = 1.f / scale;
     for (int base = 0; base < n; base += piece) {
       if (n > piece) load(base);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (base + u * RPI >= n) break;  // (uniform)
+        if (base + (u * rw + wr) * RPI >= n) break;  // (uniform)
         float y[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -334,7 +353,7 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = Grid8<F>::limit(y[e]);
         }
-        if (mine && base + u * RPI + lr < n)
+        if (mine && base + (u * rw + wr) * RPI + lr < n)
           *(u32x2*)(rows + (int64_t)(at[u] - blk * a.scale_block) * p_ss) = u32x2{Grid8<F>::pack(y), Grid8<F>::pack(y + 4)};
       }
     }
@@ -345,8 +364,9 @@ __global__ void __launch_bounds__(256) fa_kv_write_kernel(const WArgs a) {
 using namespace fa::kvhost;
 
 template <typename T, int F>
-int launch_write(const WArgs& a, int64_t units, hipStream_t st) {
-  hipLaunchKernelGGL((fa_kv_write_kernel<T, F>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
+int launch_write(const WArgs& a, int64_t wgs, int waves, hipStream_t st) {
+  if (waves > 1) hipLaunchKernelGGL((fa_kv_write_kernel<T, F, 4>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((fa_kv_write_kernel<T, F, 1>), dim3((unsigned)wgs), dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
@@ -400,10 +420,11 @@ int fa_kv_write_launch(const fa_kv_write_params* p, void* stream) {
   a.tokens = p->tokens; a.heads = p->heads; a.head_dim = p->head_dim;
   a.scale_block = (uint32_t)p->scale_block; a.blocks_per_page = (uint32_t)(p->page_size / p->scale_block);
   a.chunk = write_chunk(p);
-  const int64_t units = write_units(p);
+  const int waves = write_waves(p);
+  const int64_t wgs = write_wgs(p);
   hipStream_t st = (hipStream_t)stream;
-  if (p->dtype == FA_DTYPE_BF16) return p->format == FA_KV_E4M3 ? launch_write<__bf16, FA_KV_E4M3>(a, units, st) : launch_write<__bf16, FA_KV_INT8>(a, units, st);
-  return p->format == FA_KV_E4M3 ? launch_write<_Float16, FA_KV_E4M3>(a, units, st) : launch_write<_Float16, FA_KV_INT8>(a, units, st);
+  if (p->dtype == FA_DTYPE_BF16) return p->format == FA_KV_E4M3 ? launch_write<__bf16, FA_KV_E4M3>(a, wgs, waves, st) : launch_write<__bf16, FA_KV_INT8>(a, wgs, waves, st);
+  return p->format == FA_KV_E4M3 ? launch_write<_Float16, FA_KV_E4M3>(a, wgs, waves, st) : launch_write<_Float16, FA_KV_INT8>(a, wgs, waves, st);
 }
 
 }  // extern "C"
