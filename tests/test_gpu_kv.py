@@ -567,14 +567,6 @@ def test_attention_refusals():
             tm.paged_attention(**{**ok, **over})
 
 
-def test_write_of_keys_and_values_to_one_place_is_refused():
-    kp, vp, ks, vs, _ = (t.to(DEV) for t in _cache_for([64], 64, 2, 64, 64, F8, 173))
-    x, slot = torch.zeros(1, 2, 64, dtype=BF, device=DEV), ints([0], torch.int64)
-    for args in ((kp, kp, ks, vs), (kp, vp, ks, ks)):
-        with pytest.raises(RuntimeError, match="of their own"):
-            tm.paged_cache_write(x, x, *args, slot)
-
-
 def test_cache_tensors_that_want_gradients_are_refused():
     """Neither operator has a gradient, so a scale that requires one would get none without a word."""
     kp, vp, ks, vs, table = (t.to(DEV) for t in _cache_for([64], 64, 2, 64, 64, F8, 172))

@@ -167,13 +167,6 @@ def test_attention_beyond_one_launch_is_refused(over):
     assert capi_kv.lib().fa_kv_attn_launch(ctypes.byref(p), None, 0, None) == UNS
 
 
-@pytest.mark.parametrize("over", [dict(value_pages=0x10000), dict(value_scales=0x30000)])
-def test_writes_of_keys_and_values_to_one_place_are_refused(over):
-    L, p = capi_kv.lib(), _write(**over)
-    assert L.fa_kv_write_validate(ctypes.byref(p)) == BAD
-    assert L.fa_kv_write_launch(ctypes.byref(p), None) == BAD
-
-
 def test_attention_workspace():
     """Partial results (an fp32 row, its maximum and sum) of every query row and slice; short workspaces are refused."""
     L = capi_kv.lib()

@@ -175,7 +175,6 @@ void paged_cache_write(const at::Tensor& key, const at::Tensor& value, const at:
   const c10::OptionalDeviceGuard guard(dev);
   fill_pool(p, key_pages, value_pages, key_scales, value_scales, key.size(1), key.size(2), dev);
   if (key.size(0) == 0) return;
-  TORCH_CHECK(p.key_pages != p.value_pages && p.key_scales != p.value_scales, "keys and values must have pages and scales of their own");
   const at::Tensor k = aligned_rows(key), v = aligned_rows(value);
   p.key = k.data_ptr();
   p.value = v.data_ptr();

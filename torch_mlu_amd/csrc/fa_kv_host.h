@@ -98,7 +98,6 @@ inline int write_validate(const fa_kv_write_params* p) {
   if (const int rc = pool_validate(p)) return rc;
   if ((int64_t)p->num_pages * p->page_size > 0x7fffffffLL) return FA_ERR_UNSUPPORTED;
   if (p->heads > 65535) return FA_ERR_UNSUPPORTED;
-  if (p->key_pages == p->value_pages || p->key_scales == p->value_scales) return FA_ERR_BAD_ARG;  // two rows for one place
   if (p->tokens > 0 && (!p->key || !p->value || !p->slots)) return FA_ERR_BAD_ARG;
   if (misaligned(p->key, 16) || misaligned(p->value, 16) || misaligned(p->slots, 8)) return FA_ERR_BAD_ARG;
   const int64_t st[] = {p->key_stride_t, p->key_stride_h, p->value_stride_t, p->value_stride_h};
