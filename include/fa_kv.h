@@ -74,7 +74,8 @@ FA_API int fa_kv_plan_launch(const fa_kv_plan_params* p, void* stream);
  * Write rows into the cache.  Row t of key / value ([tokens][heads][head_dim], elements of `dtype`) goes to slot slots[t];
  * a slot below 0 or beyond the pool leaves its row out.  The rows of one call that go to one block of scale_block tokens
  * stand next to each other in the call and no slot is given twice, as fa_kv_plan_launch lays them out (other orders leave
- * the contents of such a block undefined, and nothing else).  For each block and head that rows go to:
+ * the contents of such a block undefined, and nothing else).  The same goes for one pool given for keys and values alike.  For
+ * each block and head that rows go to:
  *   needed = e4m3: 2^e, the smallest e >= -100 with 448 x 2^e >= the rows' largest finite magnitude (2^-100 without one)
  *            int8: max(largest finite magnitude x fp32(1 / 127), 2^-100)
  *   scale  = max(old scale, needed); needed alone where a row goes to the block's first slot: the block starts anew then,

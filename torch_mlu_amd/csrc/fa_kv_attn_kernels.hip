@@ -74,7 +74,7 @@ __device__ __forceinline__ bool take_nan(unsigned& w) {
 //     which are the keys of its own scores, so P needs no exchange; byte i of a lane goes to the product that makes rows
 //     d = VB L + i, and two keys' bytes are put side by side before they are converted.
 // So K and V pass through no LDS, and a wavefront's next block is on its way while it computes.  Bound by reading the cache: 64
-// sequences of 8192 keys, 32 / 8 heads, head_dim 128, e4m3: 187 us, 5.5 TB/s.  What was tried for it and changed nothing: two
+// sequences of 8192 keys, 32 / 8 heads, head_dim 128, e4m3: 188 us, 5.5 TB/s.  What was tried for it and changed nothing: two
 // blocks on their way a wavefront (twice the registers, half the wavefronts), K pieces in whole cache lines an instruction.
 //
 // A row of a token and head has only 128 bytes at head_dim 128, and memory is read at its full rate only where neighbours
@@ -430,13 +430,13 @@ __device__ __forceinline__ ArgsPtr args_again() {
   return p;
 }
 
-// Many rows against the cache, more than 32 a kv head (chunks of prompts, packed batches): MFMA-bound.  One workgroup owns 128 (query row, head of the
-// group) pairs of one (sequence, kv head), 32 a wavefront, and goes through the keys in tiles of 64.  A tile is loaded into
-// registers while the one before it is computed, converted once for all four wavefronts and kept in LDS as bf16 / fp16, double
+// Many rows against the cache, more than 32 a kv head (chunks of prompts, packed batches): MFMA-bound.  One workgroup owns 128
+// (query row, head of the group) pairs of one (sequence, kv head), 32 a wavefront, and goes through the keys in tiles of 64.  A
+// tile is loaded into registers while the one before it is computed, converted once for all four wavefronts and kept in LDS as bf16 / fp16, double
 // buffered; S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 with one lane a row, as in the 16-bit tile kernel, whose LDS
 // layouts these are.  The heads of a group share the tile, so a conversion serves 4 x 32 rows instead of one wavefront's.
 // Bound by the issue of matrix and vector instructions, which add up: 500 rows over 32768 keys, 32 / 8 heads, head_dim 128, e4m3:
-// 314 us with the join of 4 slices, 850 TFLOP/s; a wavefront's tile is 32 products (1000 cycles) and about 230 vector
+// 321 us with the join of 4 slices, 831 TFLOP/s; a wavefront's tile is 32 products (1000 cycles) and about 240 vector
 // instructions (1200), of which the conversion, 32 + 8 stores, is a sixth; both together take 2400.
 template <typename T, int F, int DP>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(const AArgs a) {

@@ -143,8 +143,8 @@ inline int64_t attn_rows(const fa_kv_attn_params* p) { return p->cu_seqlens_q ? 
 // Slices of the tile kernel: two workgroups share a CU (one at head_dim 256), and one that has it to itself takes two thirds of
 // the time; a start and an end cost about 5 tiles, the join of the slices 2 and its partial results' bytes, of which 11 MB pass
 // while a tile is computed.  Measured (us, bf16, 32 / 8 heads, head_dim 128, e4m3; in the chosen number of slices, in one, in the
-// nearest others): 500 rows over 32768 keys 324 in 4 (829; 399 in 3, 344 in 6), 4 x 512 over 4096 168 in 1 (178 in 2), packed
-// prompts and decodes 16 x 512 over 4096 198 in 2 (206; 201 in 3), 4 x 512 over 16384 212 in 3 (423; 298 in 2, 232 in 4).
+// nearest others): 500 rows over 32768 keys 317 in 4 (845; 405 in 3, 340 in 6), 4 x 512 over 4096 168 in 1 (178 in 2), packed
+// prompts and decodes 16 x 512 over 4096 181 in 2 (213; 187 in 3), 4 x 512 over 16384 212 in 3 (423; 298 in 2, 232 in 4).
 inline int64_t tile_slices(int64_t units, int64_t tiles, int64_t rows, int head_dim) {
   const double slots = head_dim > 128 ? 256 : 512;
   double least = 0;

@@ -63,7 +63,7 @@ struct Io {
 // The angles of a token's pairs are the same for all its heads: a workgroup works them out once for its tokens, in LDS, and
 // then only moves data.  An angle is formed in turns in 64 bits and its whole turns dropped there, so that it is as exact far
 // into a long prompt as at its start (in 32 bits position 10^6 would be off by 0.06 rad); sine and cosine are 32 bits of that.
-// Bound by memory: 16384 tokens of 16 + 16 heads, head_dim 128, bf16: 61 us, 4.4 TB/s read and written, of 4.95 that a copy reaches.
+// Bound by memory: 16384 tokens of 16 + 16 heads, head_dim 128, bf16: 57 us, 4.7 TB/s read and written, of 4.95 that a copy reaches.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) fa_rope_kernel(const RArgs a) {
   extern __shared__ __attribute__((aligned(16))) float2 table[];  // [per_wg][pairs]: cos, sin

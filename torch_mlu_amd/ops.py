@@ -98,7 +98,7 @@ def paged_cache_write(key, value, key_pages, value_pages, key_scales, value_scal
     finite magnitude of the new rows needs, and where it grows the block's other rows are rounded again.  A row for a block's
     first token starts the block anew.  Infinities are stored as the largest magnitude, NaN as NaN (int8: 0).  The rows of a
     call that go to one block stand next to each other and no slot is given twice, as in paged_plan's slots; otherwise such a
-    block's contents are undefined.  Inference only."""
+    block's contents are undefined, and so are those of one pool given for keys and values alike.  Inference only."""
     torch.ops.torch_mlu_amd.paged_cache_write(key, value, key_pages, value_pages, key_scales, value_scales, slots)
 
 
