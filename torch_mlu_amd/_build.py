@@ -119,8 +119,7 @@ def build_kv(verbose: bool = False) -> str:
                                     stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
              for src, obj in zip(KV_SOURCES, objs)]
     log = ""
-    for src, pr in procs:
-        o, _ = pr.communicate()
+    for src, pr, o in [(src, pr, pr.communicate()[0]) for src, pr in procs]:  # all of them end before one's error is raised
         o = "\n".join(l for l in o.splitlines() if "is not a recognized feature for this target" not in l)
         if pr.returncode != 0:
             raise RuntimeError("build step failed: hipcc -c " + src + "\n" + o)
