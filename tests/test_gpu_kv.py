@@ -367,6 +367,20 @@ def test_attention_packed(dtype, form, D, heads, kv_heads):
     _check_attention(q, kp, vp, ks, vs, table, lens, False, cu=cu, max_q=130)
 
 
+@pytest.mark.parametrize("B", [1, 64, 65, 130])
+def test_attention_packed_batches_of_every_kind(B):
+    """No rows, one, as many as a wavefront of the tile kernel holds, one more, a block and its neighbours; both ways to find a
+    sequence, in one slice and in several (few heads and long tables)."""
+    g = np.random.RandomState(B)
+    new = [int(x) for x in g.choice((0, 1, 1, 1, 8, 9, 31, 32, 33, 64, 130), B)]
+    new[-1] = 150
+    for keys, heads, kv_heads in ((200, 8, 2), (3000 if B > 1 else 9000, 4, 1)):
+        lens = [max(n, int(g.randint(1, keys))) for n in new]
+        cu = [0] + [int(x) for x in np.cumsum(new)]
+        kp, vp, ks, vs, table = _cache_for(lens, 64, kv_heads, 64, 64, F8, 75)
+        _check_attention(_q((cu[-1], heads, 64), BF, 16), kp, vp, ks, vs, table, lens, True, cu=cu, max_q=150)
+
+
 def test_attention_packed_leaves_other_rows_alone():
     """C ABI: rows behind the last sequence, and rows beyond seqlen_q, keep what they hold; cu_seqlens beyond the rows are clipped."""
     import ctypes

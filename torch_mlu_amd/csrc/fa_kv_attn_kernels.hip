@@ -458,7 +458,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
   int b, hk, split, rb;
   if (a.cu_q) {
     // The sequences' blocks of 128 rows share the grid without a place for blocks that a shorter one has not (a workgroup that
-    // exits takes its LDS for a microsecond or two, and the ones behind it wait): with c rows before it, sequence b begins at
+    // exits takes its LDS for a microsecond or two, and the ones behind it wait).  Up to 64 sequences: the blocks one after the
+    // other, those of few rows (single tokens) behind all others, where they fill the gaps of the last round (16 x 512 over
+    // 4096 213 -> 178 us in one slice, 16 / 16 heads, 6 x 2000 over 4000 143 -> 130).  More: with c rows before it, sequence b begins at
     // place c * group / 128 + b, which leaves room for its blocks and at most one place too many.
     const unsigned nhs = (unsigned)(a.heads_k * a.n_splits);
     unsigned hs, place;
@@ -470,16 +472,35 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) fa_kv_tile_kernel(cons
       place = blockIdx.x / nhs;
       hs = blockIdx.x - place * nhs;
     }
-    ConstI32Ptr cu = (ConstI32Ptr)(uintptr_t)a.cu_q;
-    auto begin = [&](int i) { return (unsigned)((uint64_t)min(max(cu[i], 0), a.total_q) * (unsigned)a.group / BM) + (unsigned)i; };
-    int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before this place
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (begin(mid) <= place) lo = mid;
-      else hi = mid - 1;
+    if (a.batch <= 64) {  // lane i looks at sequence i
+      const QRows of_lane = query_rows(a.cu_q, min(lane, a.batch - 1), a.seqlen_q, a.total_q);
+      const unsigned R = lane < a.batch ? (unsigned)of_lane.count * (unsigned)a.group : 0, n = (R + BM - 1) / BM;
+      const bool few = R > 0 && R <= 32;  // one wavefront's
+      unsigned end = few ? 0 : n;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const unsigned y = (unsigned)__shfl_up((int)end, d);
+        if (lane >= d) end += y;
+      }
+      const uint64_t fews = __ballot(few);
+      const unsigned others = (unsigned)__builtin_amdgcn_readlane((int)end, 63);
+      const unsigned first = few ? others + (unsigned)__popcll(fews & ((1ULL << lane) - 1)) : end - n;
+      const uint64_t here = __ballot(place >= first && place - first < n);
+      if (!here) return;
+      b = __builtin_ctzll(here);
+      rb = (int)(place - (unsigned)__builtin_amdgcn_readlane((int)first, b));
+    } else {
+      ConstI32Ptr cu = (ConstI32Ptr)(uintptr_t)a.cu_q;
+      auto begin = [&](int i) { return (unsigned)((uint64_t)min(max(cu[i], 0), a.total_q) * (unsigned)a.group / BM) + (unsigned)i; };
+      int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before this place
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (begin(mid) <= place) lo = mid;
+        else hi = mid - 1;
+      }
+      b = lo;
+      rb = (int)(place - begin(lo));
     }
-    b = lo;
-    rb = (int)(place - begin(lo));
     hk = (int)(hs / (unsigned)a.n_splits);
     split = (int)(hs - (unsigned)hk * a.n_splits);
   } else {

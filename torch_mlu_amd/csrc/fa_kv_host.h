@@ -143,16 +143,19 @@ inline int64_t attn_rows(const fa_kv_attn_params* p) { return p->cu_seqlens_q ? 
 // Slices of the tile kernel: two workgroups share a CU (one at head_dim 256), and one that has it to itself takes two thirds of
 // the time; a start and an end cost about 5 tiles, the join of the slices 2 and its partial results' bytes, of which 11 MB pass
 // while a tile is computed.  Measured (us, bf16, 32 / 8 heads, head_dim 128, e4m3; in the chosen number of slices, in one, in the
-// nearest others): 500 rows over 32768 keys 317 in 4 (845; 405 in 3, 340 in 6), 4 x 512 over 4096 168 in 1 (178 in 2), packed
-// prompts and decodes 16 x 512 over 4096 181 in 2 (213; 187 in 3), 4 x 512 over 16384 212 in 3 (423; 298 in 2, 232 in 4).
-inline int64_t tile_slices(int64_t units, int64_t tiles, int64_t rows, int head_dim) {
+// nearest others): 500 rows over 32768 keys 317 in 4 (845; 405 in 3, 340 in 6), 4 x 512 over 4096 168 in 1 (178 in 2), 4 x 512 over
+// 16384 212 in 3 (423; 298 in 2, 232 in 4).  Packed batches of prompts and single tokens have lengths of all sizes, so that rounds
+// run into one another: six tenths of their number, and half of a longest block at the end.  16 x 512 over 4096 176 in 1 (183 in 2),
+// 64 x 256 over 2048 167 in 1 (203 in 2), 28 / 4 heads, 8 x 1024 over 8192 262 in 3 (261; 273 in 2), 16 / 4 heads, 40 x 300 over
+// 6000 180 in 3 (190; 188 in 2, 171 in 4), 16 / 16 heads, 6 x 2000 over 4000 130 in 1 (143 in 2).
+inline int64_t tile_slices(int64_t units, int64_t tiles, int64_t rows, int head_dim, bool packed) {
   const double slots = head_dim > 128 ? 256 : 512;
   double least = 0;
   int64_t best = 1;
   for (int64_t n = 1; n <= FA_MAX_SPLITS && (n == 1 || tiles >= 2 * n); ++n) {
     const double x = (double)units * (double)n / slots, whole = floor(x), part = x - whole;
-    const double rounds = whole + (part == 0 ? 0 : (part <= 0.5 ? 0.66 : 1));
-    const double cost = rounds * ((double)tiles / (double)n + 5) + (n > 1 ? 2 + (double)rows * (double)n * (8.0 * head_dim + 16) / 11e6 : 0);
+    const double rounds = packed ? (x > 0.83 ? 0.6 * x + 0.5 : 1) : whole + (part == 0 ? 0 : (part <= 0.5 ? 0.66 : 1));
+    const double cost = rounds * ((double)tiles / (double)n + 5) + (n > 1 ? (packed ? 8 : 2) + (double)rows * (double)n * (8.0 * head_dim + 16) / 11e6 : 0);
     if (n == 1 || cost < least) {
       least = cost;
       best = n;
@@ -197,7 +200,9 @@ inline AttnPlan attn_plan(const fa_kv_attn_params* p) {
     // (packed: a sequence with c rows before it begins at place c * group / 128 + its number)
     const int64_t places = p->cu_seqlens_q ? (int64_t)p->total_q * group / 128 + p->batch : (rows + 127) / 128;
     r.row_blocks = places > 0x7fffffff ? 0x7fffffff : (int32_t)places;
-    if (n == 0) n = tile_slices((p->cu_seqlens_q ? places : places * p->batch) * p->heads_k, blocks, attn_rows(p) * p->heads_q, p->head_dim);
+    // (blocks of few rows count half: they fill the gaps that the others leave)
+    const int64_t units = p->cu_seqlens_q ? (int64_t)p->total_q * group / 128 + p->batch / 2 : places * p->batch;
+    if (n == 0) n = tile_slices((units > 0 ? units : 1) * p->heads_k, blocks, attn_rows(p) * p->heads_q, p->head_dim, p->cu_seqlens_q != nullptr);
   } else {
     const int dp = p->head_dim <= 64 ? 64 : (p->head_dim <= 128 ? 128 : 256), waves = stream_waves(dp);
     r.hw_log2 = p->heads_k % 2 == 0 ? 1 : 0;
